@@ -46,7 +46,14 @@ extern "C" {
 #define TH_RUNTIME_ERROR 6         /* HalError::RuntimeError */
 
 /* ---- element types: TileDtype (crates/tile_hal/src/kernel.rs:84-93) ---- */
-typedef enum th_dtype { TH_F32 = 0, TH_F16 = 1, TH_BF16 = 2 } th_dtype;
+typedef enum th_dtype {
+  TH_F32 = 0,
+  TH_F16 = 1,
+  TH_BF16 = 2,
+  /* 8-bit types of a paged cache (section 2); no other entry point takes them */
+  TH_E4M3 = 3, /* 4 exponent and 3 mantissa bits, no infinities, largest value 448 */
+  TH_I8 = 4    /* whole numbers; the cache holds -127 .. 127 */
+} th_dtype;
 
 /* ---- kernel modes: KernelMode (crates/tile_hal/src/kernel.rs:8-17) ---- */
 typedef enum th_kernel_mode { TH_MODE_VECTOR = 0, TH_MODE_MATRIX = 1, TH_MODE_GENERAL = 2 } th_kernel_mode;
@@ -239,6 +246,106 @@ int th_attention_decode_static(const void* q, const void* k, const void* v, void
                                uint32_t batch, uint32_t seq_len, uint32_t max_seq,
                                uint32_t head_dim, uint32_t num_heads, uint32_t num_kv_heads,
                                th_dtype dtype, th_stream s);
+
+/* ---- paged cache, and attention over it -----------------------------------------------
+ * The kernels a serving step needs around th_attention_*: K and V in pages of a pool, the
+ * sequences of a batch of any lengths, each with any number of new tokens.  No counterpart in
+ * the reference's runtime (its __tile_attention_decode_f32 and __tile_attention_prefill_f32,
+ * tile.rs:2124, :2136, read one contiguous cache; causality, head groups and the 1/sqrt(D)
+ * scale here are theirs).
+ *
+ * th_kv_pages: the pool.  K and V are [num_pages][num_kv_heads][page_size][head_dim] in `dtype`
+ * (F16, BF16, E4M3 or I8), consecutive pages page_stride elements apart in both (0: dense).
+ * E4M3 and I8 hold codes, with one f32 scale for each page, head and position in k_scale and
+ * v_scale, dense [num_pages][num_kv_heads][page_size] (NULL otherwise): value = code * scale.
+ * page_size is a power of two of 16 to 65536, head_dim a multiple of 16 up to 256, page_stride
+ * a multiple of 16 elements; every pointer is 16-byte aligned. */
+typedef struct th_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  uint64_t page_stride;
+  uint32_t num_pages;
+  uint32_t page_size;
+  uint32_t num_kv_heads;
+  uint32_t head_dim;
+  th_dtype dtype;
+} th_kv_pages;
+
+/* th_kv_batch: the sequences, in device memory.  Sequence b has kv_len[b] positions, its new
+ * tokens among them as the last ones, and its new tokens are rows q_start[b] .. q_start[b+1]-1
+ * of Q, O and of the K and V that are written (q_start[0] = 0, not falling; total_q rows lie in
+ * these tensors, and rows from q_start[batch] on are left alone).  Position p of sequence b is
+ * row p % page_size of page page_table[b * max_pages + p / page_size].  Sequences may share
+ * pages that no call writes.
+ * The contents are read by the kernels, not checked on the host.  Nothing outside the pool and
+ * the tensors is touched whatever they hold: a table entry outside [0, num_pages) is a page that
+ * is not there (not written, read as zeros, hidden from attention), as are positions past
+ * max_pages * page_size; a token whose position is negative (kv_len[b] less than its new tokens)
+ * is not written and sees nothing. */
+typedef struct th_kv_batch {
+  const int32_t* page_table; /* [batch][max_pages] */
+  const int32_t* q_start;    /* [batch + 1] */
+  const int32_t* kv_len;     /* [batch] */
+  uint32_t batch;
+  uint32_t max_pages;
+  uint32_t total_q;
+} th_kv_batch;
+
+/* Write the new tokens' K and V, [total_q][num_kv_heads][head_dim] in dtype (F32, F16 or BF16)
+ * with `stride` elements between tokens (0: dense; else at least num_kv_heads * head_dim, and
+ * whole 16-byte blocks), into the cache.  16-bit caches round to nearest even.  8-bit ones take
+ * scale = a / M for each token and head, a being the largest magnitude of its head_dim values
+ * and M 448 (E4M3) or 127 (I8), and code = x * (M / a) rounded to the nearest code, ties to
+ * even, each quotient and product rounded to f32.  Values all below 1e-30 give scale and codes
+ * of zero; a token and head with a NaN or an infinity gives codes of zero and a NaN scale, so
+ * that all of it reads as NaN.  Two tokens of one call must not share a position of a page: what
+ * that position then holds is unspecified. */
+int th_kv_cache_write(const th_kv_pages* pages, const th_kv_batch* seqs, const void* k,
+                      const void* v, uint64_t stride, th_dtype dtype, th_stream s);
+
+/* Read positions [0, kv_len[b]) of every sequence into K and V,
+ * [batch][num_kv_heads][max_seq][head_dim] in dtype (F32, F16 or BF16; code * scale is rounded
+ * to f32, then to dtype), the layout of th_attention_prefill and th_attention_decode.  Positions from max_seq on are not read, rows
+ * from kv_len[b] on are left as they were. */
+int th_kv_cache_read(const th_kv_pages* pages, const th_kv_batch* seqs, void* k, void* v,
+                     uint32_t max_seq, th_dtype dtype, th_stream s);
+
+/* Causal attention of the new tokens over their sequences' pages: the token at position p sees
+ * positions 0 .. p, its own K and V among them (write them first).  Q is
+ * [total_q][num_heads][head_dim] with q_stride elements between tokens (0: dense; else at least
+ * num_heads * head_dim and a multiple of 8), O the same, dense.  dtype is F16 or BF16; the cache
+ * is of that dtype, or E4M3 or I8.  num_heads is a multiple of num_kv_heads.  Scores, softmax
+ * and sums are f32; probabilities are rounded to dtype.  A token that sees nothing gives zeros.
+ * What a token does not see has no effect on it, NaN and infinities included.
+ * The work is split by the lengths on the device, so one captured call serves any lengths; the
+ * parts' sums go to `workspace`, device memory of at least th_attention_paged_workspace_size
+ * bytes for the same arguments (of the structs' sizes, not the lengths).  With NULL they go to
+ * the stream's scratch, which a stream that is being captured does not offer
+ * (TH_MEMORY_ERROR).  Calls that overlap on a device need workspaces of their own. */
+size_t th_attention_paged_workspace_size(const th_kv_pages* pages, const th_kv_batch* seqs,
+                                         uint32_t num_heads);
+int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batch* seqs, void* o,
+                       uint32_t num_heads, uint64_t q_stride, th_dtype dtype, void* workspace,
+                       size_t workspace_bytes, th_stream s);
+
+/* The next token of each row of logits, [rows][vocab] in dtype with `stride` elements between
+ * rows (0: vocab), from one given random number per row.  Per row, in device memory, NULL where
+ * a limit is not used: temperature (1 without), top_k, top_p, min_p; uniform is in [0, 1).
+ * With x the row, x_max its largest value and w_i = exp((x_i - x_max) / temperature), tokens are
+ * ordered by x, the largest first, equal ones by index.  Kept are: the first top_k (all where
+ * it is <= 0); of those the shortest run of at least top_p of their mass, i.e. each token with
+ * less than top_p of it before it (all where top_p >= 1 or NaN); of those the ones with
+ * w_i >= min_p; and always the first.  tokens[row] is the lowest index whose mass, with that of
+ * the kept ones of lower index, exceeds uniform * (mass of the kept).  Where temperature is <= 0
+ * or NaN that is the first of the order.  Logits of NaN and -infinity are never chosen; a row of nothing
+ * else gives -1.  Weights are f32 with steps of 2^-31 of the largest; masses are exact sums of
+ * them, so a result does not depend on the order of summation.  Cf. the reference's
+ * __tile_sample_top_p intrinsic, which its emitters print and this runtime takes no tile for. */
+int th_sample(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab, uint64_t stride,
+              th_dtype dtype, const float* uniform, const float* temperature,
+              const int32_t* top_k, const float* top_p, const float* min_p, th_stream s);
 
 /* Synthetic data: fill `n` elements with i.i.d. samples, counter-based and
  * seeded (element i depends only on (seed, i)).  dist 0 = Uniform[p0, p1),

@@ -10,7 +10,8 @@
 namespace th {
 
 // Element-type tags; numerically equal to TH_DTYPE_* in include/tilers_hip.h.
-enum Dtype : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+// (kE4M3, kI8: codes of a paged cache only.)
+enum Dtype : int { kF32 = 0, kF16 = 1, kBF16 = 2, kE4M3 = 3, kI8 = 4 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -1,0 +1,55 @@
+// th_sample (include/tilers_hip.h, section 2).
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "kernels/sample.hpp"
+#include "ops_common.hpp"
+#include "runtime.hpp"
+
+using th::fail;
+using namespace th::ops;
+
+namespace {
+
+template <int DT>
+int sample_go(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab, uint64_t stride,
+              const float* uniform, const float* temperature, const int32_t* top_k,
+              const float* top_p, const float* min_p, hipStream_t s) {
+  hipLaunchKernelGGL((th::smp::sample_rows<DT>), dim3(rows), dim3(th::smp::NT), 0, s, logits,
+                     tokens, vocab, stride, uniform, temperature, top_k, top_p, min_p);
+  return launch_status("sample launch");
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace
+
+extern "C" int th_sample(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab,
+                         uint64_t stride, th_dtype dtype, const float* uniform,
+                         const float* temperature, const int32_t* top_k, const float* top_p,
+                         const float* min_p, th_stream s) {
+  if (!valid_dtype(dtype)) return fail(TH_KERNEL_ERROR, "sample: unknown dtype");
+  if (stride == 0) stride = vocab;
+  if (stride < vocab) return fail(TH_KERNEL_ERROR, "sample: stride is less than vocab");
+  if (vocab > 0x7fffffffu || rows > 0x7fffffffu)
+    return fail(TH_KERNEL_ERROR, "sample: rows and vocab must be below 2^31");
+  if (rows == 0) return TH_OK;
+  if (vocab == 0) return fail(TH_KERNEL_ERROR, "sample: vocab == 0");
+  if (stride > (uint64_t{1} << 60) / rows) return fail(TH_KERNEL_ERROR, "sample: stride is too large");
+  if (!logits || !tokens || !uniform) return fail(TH_KERNEL_ERROR, "sample: null pointer");
+  if (!aligned(logits, dtype_size(dtype)) || !aligned(tokens, 4) || !aligned(uniform, 4) ||
+      !aligned(temperature, 4) || !aligned(top_k, 4) || !aligned(top_p, 4) || !aligned(min_p, 4))
+    return fail(TH_KERNEL_ERROR, "sample: pointers must be aligned to their elements");
+  switch (dtype) {
+    case TH_F32:
+      return sample_go<th::kF32>(logits, tokens, rows, vocab, stride, uniform, temperature, top_k,
+                                 top_p, min_p, as_stream(s));
+    case TH_F16:
+      return sample_go<th::kF16>(logits, tokens, rows, vocab, stride, uniform, temperature, top_k,
+                                 top_p, min_p, as_stream(s));
+    default:
+      return sample_go<th::kBF16>(logits, tokens, rows, vocab, stride, uniform, temperature, top_k,
+                                  top_p, min_p, as_stream(s));
+  }
+}

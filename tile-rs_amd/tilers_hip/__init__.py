@@ -29,14 +29,15 @@ from typing import Callable, Optional, Sequence
 import numpy as np
 
 from ._lib import (EMIT_FN, TH_BACKEND_NOT_AVAILABLE, TH_KERNEL_ERROR, TH_OK, EmitOpts, HalError,
-                   check, load)
+                   KvBatchStruct, KvPagesStruct, check, load)
 
 __all__ = [
     "HalError", "TileDtype", "KernelMode", "LaunchGrid", "MemInfo", "HipDevice", "HipStream",
     "HipBuffer", "HipLauncher", "HipEvent", "BackendSelector", "BackendKind", "EmitOut",
     "TargetMeta", "CodegenTarget", "EmitterTarget", "TargetRegistry", "softmax", "matmul",
     "matmul_silu_mul", "rms_norm", "causal_mask_f32", "attention", "attention_prefill", "attention_decode",
-    "attention_decode_workspace_size", "fill_random", "compile_source", "device_count", "lib",
+    "attention_decode_workspace_size", "KvPages", "KvBatch", "kv_cache_write", "kv_cache_read",
+    "attention_paged", "attention_paged_workspace_size", "sample", "fill_random", "compile_source", "device_count", "lib",
 ]
 
 
@@ -45,18 +46,22 @@ def lib():
 
 
 class TileDtype(enum.IntEnum):
-    """TileDtype subset the hot path uses (crates/tile_hal/src/kernel.rs:84-93)."""
+    """TileDtype subset the hot path uses (crates/tile_hal/src/kernel.rs:84-93), and the 8-bit
+    types of a paged cache."""
     F32 = 0
     F16 = 1
     BF16 = 2
+    E4M3 = 3
+    I8 = 4
 
     @property
     def itemsize(self) -> int:
-        return 4 if self == TileDtype.F32 else 2
+        return 4 if self == TileDtype.F32 else 2 if self <= TileDtype.BF16 else 1
 
     @property
     def host_dtype(self):
-        return np.float32 if self == TileDtype.F32 else np.uint16
+        return {TileDtype.F32: np.float32, TileDtype.E4M3: np.uint8,
+                TileDtype.I8: np.int8}.get(self, np.uint16)
 
 
 class KernelMode(enum.IntEnum):
@@ -401,6 +406,65 @@ def attention_decode(q, k, v, o, batch: int, seq_len: int, max_seq: int, head_di
     check(lib().th_attention_decode(_p(q), _p(k), _p(v), _p(o), batch, seq_len, max_seq, head_dim,
                                     num_heads, num_kv_heads, int(dtype), _p(workspace),
                                     workspace_bytes, _s(stream)))
+
+
+class KvPages:
+    """A pool of cache pages (th_kv_pages): K and V [num_pages][num_kv_heads][page_size][head_dim],
+    page_stride elements apart (0: dense), with f32 scales [num_pages][num_kv_heads][page_size]
+    where dtype is E4M3 or I8.  Holds the buffers that it is given."""
+
+    def __init__(self, k, v, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 dtype: TileDtype, k_scale=None, v_scale=None, page_stride: int = 0):
+        self._held = (k, v, k_scale, v_scale)
+        self.struct = KvPagesStruct(_p(k), _p(v), _p(k_scale), _p(v_scale), page_stride, num_pages,
+                                    page_size, num_kv_heads, head_dim, int(dtype))
+        self._ref = C.byref(self.struct)
+
+
+class KvBatch:
+    """The sequences of a call on pages (th_kv_batch): int32 device arrays page_table
+    [batch][max_pages], q_start [batch + 1] and kv_len [batch].  Holds the buffers that it is
+    given; what they hold may change from call to call."""
+
+    def __init__(self, page_table, q_start, kv_len, batch: int, max_pages: int, total_q: int):
+        self._held = (page_table, q_start, kv_len)
+        self.struct = KvBatchStruct(_p(page_table), _p(q_start), _p(kv_len), batch, max_pages,
+                                    total_q)
+        self._ref = C.byref(self.struct)
+
+
+def kv_cache_write(pages: KvPages, seqs: KvBatch, k, v, dtype: TileDtype = TileDtype.BF16,
+                   stride: int = 0, stream: Optional[HipStream] = None) -> None:
+    """The new tokens' K and V into their pages, quantised where the cache has 8 bits."""
+    check(lib().th_kv_cache_write(pages._ref, seqs._ref, _p(k), _p(v), stride, int(dtype),
+                                  _s(stream)))
+
+
+def kv_cache_read(pages: KvPages, seqs: KvBatch, k, v, max_seq: int,
+                  dtype: TileDtype = TileDtype.BF16, stream: Optional[HipStream] = None) -> None:
+    """Every sequence's cached positions into K, V [batch][num_kv_heads][max_seq][head_dim]."""
+    check(lib().th_kv_cache_read(pages._ref, seqs._ref, _p(k), _p(v), max_seq, int(dtype),
+                                 _s(stream)))
+
+
+def attention_paged_workspace_size(pages: KvPages, seqs: KvBatch, num_heads: int) -> int:
+    return lib().th_attention_paged_workspace_size(pages._ref, seqs._ref, num_heads)
+
+
+def attention_paged(q, pages: KvPages, seqs: KvBatch, o, num_heads: int,
+                    dtype: TileDtype = TileDtype.BF16, q_stride: int = 0, workspace=None,
+                    workspace_bytes: int = 0, stream: Optional[HipStream] = None) -> None:
+    """Causal attention of each sequence's new tokens over its pages."""
+    check(lib().th_attention_paged(_p(q), pages._ref, seqs._ref, _p(o), num_heads, q_stride,
+                                   int(dtype), _p(workspace), workspace_bytes, _s(stream)))
+
+
+def sample(logits, tokens, rows: int, vocab: int, dtype: TileDtype, uniform, temperature=None,
+           top_k=None, top_p=None, min_p=None, stride: int = 0,
+           stream: Optional[HipStream] = None) -> None:
+    """tokens (int32) [rows] drawn from the rows' logits with the numbers in uniform."""
+    check(lib().th_sample(_p(logits), _p(tokens), rows, vocab, stride, int(dtype), _p(uniform),
+                          _p(temperature), _p(top_k), _p(top_p), _p(min_p), _s(stream)))
 
 
 def fill_random(dst, n: int, dtype: TileDtype, dist: str, p0: float, p1: float, seed: int,

@@ -43,6 +43,18 @@ class EmitOpts(C.Structure):
     _fields_ = [("ub_size", C.c_size_t)]
 
 
+class KvPagesStruct(C.Structure):   # th_kv_pages
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("page_stride", C.c_uint64), ("num_pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("num_kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("dtype", C.c_int)]
+
+
+class KvBatchStruct(C.Structure):   # th_kv_batch
+    _fields_ = [("page_table", C.c_void_p), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("batch", C.c_uint32), ("max_pages", C.c_uint32), ("total_q", C.c_uint32)]
+
+
 EMIT_FN = C.CFUNCTYPE(C.c_int, C.c_char_p, C.c_size_t, C.POINTER(EmitOpts), _ppc, _ppc, _ppc, _ppc)
 
 SIGNATURES: dict[str, tuple] = {
@@ -93,6 +105,15 @@ SIGNATURES: dict[str, tuple] = {
                                  _sz, _vp]),
     "th_attention_decode_static": (_i, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32,
                                         _i, _vp]),
+    "th_kv_cache_write": (_i, [C.POINTER(KvPagesStruct), C.POINTER(KvBatchStruct), _vp, _vp, _u64,
+                               _i, _vp]),
+    "th_kv_cache_read": (_i, [C.POINTER(KvPagesStruct), C.POINTER(KvBatchStruct), _vp, _vp, _u32,
+                              _i, _vp]),
+    "th_attention_paged_workspace_size": (_sz, [C.POINTER(KvPagesStruct),
+                                                C.POINTER(KvBatchStruct), _u32]),
+    "th_attention_paged": (_i, [_vp, C.POINTER(KvPagesStruct), C.POINTER(KvBatchStruct), _vp,
+                                _u32, _u64, _i, _vp, _sz, _vp]),
+    "th_sample": (_i, [_vp, _vp, _u32, _u32, _u64, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "th_fill_random": (_i, [_vp, _u64, _i, _i, _f, _f, _u64, _vp]),
     "th_target_name": (_cp, []),
     "th_emit": (_i, [_cp, _sz, C.POINTER(EmitOpts), _ppc, _ppc, _ppc, _ppc]),
