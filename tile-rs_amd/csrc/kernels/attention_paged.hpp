@@ -111,18 +111,21 @@ struct AttnArgs {
   uint64_t q_stride;
   float scale_log2;
   uint32_t nh, group;
+  uint32_t split_rows;   // sequences of more rows are the chunk kernel's, the others the rows'
+  uint32_t parts;        // parts that a chunk tile's positions are cut into, at most
+  float* chunk_ws;       // the chunk kernel's sums: [parts][total_q * nh] records
 };
 
-// Work of one sequence: tiles of `tr` rows, and units of `unit` positions (one at least, so that
-// rows without any position are written too).
+// Work of one sequence: tiles of TR rows, and units of UNIT positions (one at least, so that rows
+// without any position are written too).
 struct SeqWork {
   uint32_t tiles, units;
 };
-__device__ __forceinline__ SeqWork seq_work(const PagedChunk& c, uint32_t group, uint32_t tr,
-                                            uint32_t unit) {
+__device__ __forceinline__ SeqWork rows_work(const AttnArgs& a, const PagedChunk& c) {
   SeqWork w;
-  w.tiles = (c.n * group + tr - 1) / tr;
-  const uint32_t u = c.held / unit + (c.held % unit != 0);
+  const uint32_t r = c.n * a.group;   // the host keeps total_q * num_heads below 2^31
+  w.tiles = r <= a.split_rows ? (r + rows::TR - 1) / rows::TR : 0u;
+  const uint32_t u = c.held / rows::UNIT + (c.held % rows::UNIT != 0);
   w.units = u == 0 ? 1u : u;
   return w;
 }
@@ -152,7 +155,7 @@ __device__ __forceinline__ uint64_t scan_units(const AttnArgs& a, F&& visit) {
   for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
     uint64_t u = 0;
     if (b0 + lane < a.seqs.batch) {
-      const SeqWork w = seq_work(paged_chunk(a.seqs, b0 + lane), a.group, rows::TR, rows::UNIT);
+      const SeqWork w = rows_work(a, paged_chunk(a.seqs, b0 + lane));
       u = static_cast<uint64_t>(w.tiles) * w.units * a.pool.nkv;
     }
     uint64_t inc = u;
@@ -235,8 +238,10 @@ struct RowsTile {
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < KL / 2; ++i) {
-        const uint32_t c = min(static_cast<uint32_t>(64 * i + 16 * g), rb - 16);
-        st.k[t * (KL / 2) + i] = ldg128_nt(kp + at[t] + l16 * rb + c);
+        const uint32_t c = 64 * i + 16 * g;
+        u32x4& k = st.k[t * (KL / 2) + i];
+        k = ldg128_nt(kp + at[t] + l16 * rb + min(c, rb - 16));
+        if (c >= rb) k = u32x4{0, 0, 0, 0};   // (Q is zero there, K may be infinite)
       }
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
@@ -315,7 +320,7 @@ struct RowsTile {
     const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t D = a.pool.head_dim, G = a.group;
-    const uint32_t nrows = c.n * G;   // the host keeps total_q * num_heads below 2^31
+    const uint32_t nrows = c.n * G;
     const uint32_t row = tile * rows::TR + l16;
     const bool live_row = row < nrows;
     const uint32_t qi = row / G, hq = h * G + row % G;
@@ -393,16 +398,15 @@ struct RowsTile {
 #pragma unroll
         for (int i = 0; i < 8; ++i) vs[i] = hid[i >> 2][i & 3] ? 0.0f : cur.vs[i >> 2][i & 3];
         if constexpr (DT == kF16) {
-          // f16 has five exponent bits: the scales enter relative to a power of two not far
-          // below their largest so far
+          // f16 has five exponent bits: the scales enter relative to a power of two just above
+          // the largest that the row has seen
           float big = vs[0];
 #pragma unroll
           for (int i = 1; i < 8; ++i) big = fmaxf(big, vs[i]);
           int e = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000;
           if (__builtin_amdgcn_ballot_w64(e > ev) != 0) {
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) e = max(e, __shfl_xor(e, o));
-            e = max(e, ev);
+            e = max(e, __shfl_xor(e, 16));
+            e = max(max(e, __shfl_xor(e, 32)), ev);
             alpha *= __builtin_ldexpf(1.0f, max(ev - e, -300));
             ev = e;
             moved = true;
@@ -545,7 +549,7 @@ attn_paged_rows(AttnArgs a) {
   Where at = find_unit(a, u);
   while (u < u1 && at.b < a.seqs.batch) {
     const PagedChunk c = paged_chunk(a.seqs, at.b);
-    const SeqWork sw = seq_work(c, a.group, rows::TR, rows::UNIT);
+    const SeqWork sw = rows_work(a, c);
     const uint64_t all = static_cast<uint64_t>(sw.tiles) * sw.units * a.pool.nkv;
     if (all == 0) {
       ++at.b;
@@ -584,7 +588,7 @@ attn_paged_merge(AttnArgs a, uint32_t nw) {
   const Where at = find_unit(a, u);
   if (at.b >= a.seqs.batch) return;
   const PagedChunk c = paged_chunk(a.seqs, at.b);
-  const SeqWork sw = seq_work(c, a.group, rows::TR, rows::UNIT);
+  const SeqWork sw = rows_work(a, c);
   const uint64_t in = u - at.before;
   const uint64_t item0 = u - in % sw.units, item1 = item0 + sw.units;
   if (item0 == u || run_start(units, w, nw) > item0) return;
@@ -629,6 +633,536 @@ attn_paged_merge(AttnArgs a, uint32_t nw) {
     }
     if (pg == 0 && c8 < static_cast<int>(a.pool.head_dim))
       T::write_row(a, c, h, r0 + r, c8, o, ls);
+  }
+}
+
+// ---- the chunks' kernel: tiles of 256 rows ------------------------------------------------
+//
+// For many new tokens, which are bound by the matrix cores.  One workgroup of 8 waves per (tile,
+// kv head, part of the positions), 32 rows a wave; 64 positions at a time go through LDS, double-
+// buffered, as 16-bit values (codes are widened on the way in, once for all eight waves).  Per
+// wave and block:
+//   S^T (64 x 32) = K . Q^T     2 x HD/16 32x32x16 MFMAs, Q^T in registers
+//   O^T (HD x 32) += V^T . P^T  4 x HD/32 MFMAs; P^T is S^T's accumulator converted in place,
+//                               the transposing read of V gives V^T in the same order
+// Where there are fewer (tile, head) items than CUs the positions are cut into parts, which
+// chunk_merge adds up.
+namespace chunk {
+constexpr int NT = 512;
+constexpr int TR = 256;
+constexpr int KB = 64;           // positions of a block
+constexpr uint32_t kLeast = 8;   // blocks of a part, at least
+__host__ __device__ constexpr int rec(int hd) { return hd + 4; }   // O, then l, m
+
+// Tiles of a sequence, and the blocks of each part of one whose last row sees `vis` positions.
+__device__ __forceinline__ uint32_t tiles(const AttnArgs& a, const PagedChunk& c) {
+  const uint32_t r = c.n * a.group;
+  return r > a.split_rows ? (r + TR - 1) / TR : 0u;
+}
+__device__ __forceinline__ uint32_t part_blocks(uint32_t vis, uint32_t parts) {
+  const uint32_t nb = (vis + KB - 1) / KB;
+  return max(kLeast, (nb + parts - 1) / parts);
+}
+// Positions that the tile's last row sees.
+__device__ __forceinline__ uint32_t tile_reach(const AttnArgs& a, const PagedChunk& c,
+                                               uint32_t tile) {
+  const uint32_t r1 = min(c.n * a.group, (tile + 1) * TR) - 1;
+  return paged_visible(c, r1 / a.group);
+}
+}  // namespace chunk
+
+// max (sum) of a lane's value and that of the lane 32 away
+__device__ __forceinline__ float pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int DT, int CT, int HD>
+struct ChunkTile {
+  static_assert(HD == 64 || HD == 128, "chunk kernel head dim");
+  static constexpr bool kCodes = cache_codes<CT>();
+  static constexpr int ESZ = cache_size<CT>();
+  static constexpr int RB = HD * 2;                  // bytes of a row in LDS
+  static constexpr int KBYTES = chunk::KB * RB;      // of a block's K (or V)
+  static constexpr int CPR = HD * ESZ / 16;          // 16-byte pieces of a row in memory
+  static constexpr int NX = chunk::KB * CPR;         // of a block
+  static constexpr int XPT = (NX + chunk::NT - 1) / chunk::NT;   // per thread
+  static constexpr int NDS = HD / 16, NDT = HD / 32;
+
+  struct Lds {
+    char kv[2][2 * KBYTES];
+    float ks[2][chunk::KB], vs[2][chunk::KB];   // 0 where nothing is held
+    uint32_t there[2][4];                       // the pages of the block's four groups exist
+    uint32_t odd[2];                            // the block with NaN or infinities in V
+  };
+  struct Stage {
+    u32x4 k[XPT], v[XPT];
+    float scale;
+  };
+
+  // LDS layouts without bank conflicts: K in halves of 64 columns, chunk c of row r at
+  // c ^ f(r), where a read of 32 rows' chunks meets every bank evenly; V as for the rows' kernel.
+  static __device__ __forceinline__ uint32_t kswz(uint32_t r) {
+    return ((r >> 1) & 3u) | ((r >> 2) & 4u);
+  }
+  static __device__ __forceinline__ uint32_t kaddr(uint32_t r, uint32_t c) {
+    return (c >> 3) * (chunk::KB * 128) + r * 128 + (((c & 7) ^ kswz(r)) << 4);
+  }
+  static __device__ __forceinline__ uint32_t vswz(uint32_t r) {
+    return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
+  }
+  static __device__ __forceinline__ uint32_t vaddr(uint32_t r, uint32_t c) {
+    return r * RB + ((c ^ vswz(r)) << 4);
+  }
+};
+
+template <int DT, int CT, int HD>
+__global__ void __launch_bounds__(chunk::NT)
+attn_paged_chunk(AttnArgs a) {
+  using T = ChunkTile<DT, CT, HD>;
+  using namespace chunk;
+  constexpr int XPT = T::XPT;
+  __shared__ __align__(16) typename T::Lds sh;
+  const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, g = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint32_t nkv = a.pool.nkv, D = a.pool.head_dim, G = a.group;
+
+  // item: heads fastest (workgroup w runs on XCD w % 8, so a head's tiles share an L2 where
+  // there are eight), then parts, then tiles from the last (longest) on, then sequences
+  const uint32_t h = blockIdx.x % nkv;
+  const uint32_t part = blockIdx.x / nkv % a.parts;
+  uint32_t left = blockIdx.x / nkv / a.parts, b = 0;
+  {
+    bool found = false;
+    for (uint32_t b0 = 0; b0 < a.seqs.batch && !found; b0 += 64) {
+      const uint32_t n =
+          b0 + lane < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, b0 + lane)) : 0u;
+      uint32_t inc = n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t x = __shfl_up(inc, d);
+        if (lane >= d) inc += x;
+      }
+      const uint64_t in = __builtin_amdgcn_ballot_w64(left < inc);
+      if (in != 0) {
+        const int l = __builtin_ctzll(in);
+        b = b0 + l;
+        // tiles of this sequence from the last
+        left = __builtin_amdgcn_readlane(static_cast<int>(inc), l) - 1 - left;
+        found = true;
+      } else {
+        left -= __builtin_amdgcn_readlane(static_cast<int>(inc), 63);
+      }
+    }
+    if (!found) return;
+  }
+  const uint32_t tile = __builtin_amdgcn_readfirstlane(left);
+  const PagedChunk c = paged_chunk(a.seqs, b);
+  const uint32_t nrows = c.n * G;
+  const uint32_t reach = __builtin_amdgcn_readfirstlane(tile_reach(a, c, tile));
+  const uint32_t per = part_blocks(reach, a.parts);
+  const uint32_t nb_all = (reach + KB - 1) / KB;
+  const uint32_t j0 = part * per, j1 = min(nb_all, j0 + per);
+  if (part != 0 && j0 >= nb_all) return;
+  const bool whole = per >= nb_all;
+
+  // the wave's rows, and what they see
+  const uint32_t wr0 = tile * TR + wave * 32;
+  const uint32_t row = wr0 + l32;
+  const bool live_wave = wr0 < nrows, live_row = row < nrows;
+  const uint32_t qi = live_row ? row / G : 0u, hq = h * G + (live_row ? row % G : 0u);
+  const uint32_t vis = live_row ? paged_visible(c, qi) : 0u;
+  const uint32_t vis_min =
+      live_wave ? __builtin_amdgcn_readfirstlane(paged_visible(c, wr0 / G)) : 0u;
+  const uint32_t vis_max =
+      live_wave ? __builtin_amdgcn_readfirstlane(paged_visible(c, (min(nrows, wr0 + 32) - 1) / G))
+                : 0u;
+  const uint32_t tile_min =
+      __builtin_amdgcn_readfirstlane(paged_visible(c, tile * TR / G));
+
+  u32x4 qf[T::NDS];
+#pragma unroll
+  for (int s = 0; s < T::NDS; ++s) {
+    qf[s] = u32x4{0, 0, 0, 0};
+    if (live_row && 16u * s + 8u * g < D)
+      qf[s] = ldg128(a.q + (c.first + qi) * a.q_stride + static_cast<uint64_t>(hq) * D + 16 * s +
+                     8 * g);
+  }
+  f32x16 acc[T::NDT];
+#pragma unroll
+  for (int i = 0; i < T::NDT; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  int ev = -1000;   // f16 with codes: O is in units of 2^ev
+  if (t < 2) sh.odd[t] = 0xffffffffu;
+
+  // this thread's pieces of a block: rows xr, 16-byte pieces xc
+  uint32_t xr[XPT], xc[XPT];
+#pragma unroll
+  for (int i = 0; i < XPT; ++i) {
+    const uint32_t x = min(static_cast<uint32_t>(t + NT * i), static_cast<uint32_t>(T::NX - 1));
+    xr[i] = x / T::CPR;
+    xc[i] = x % T::CPR;
+  }
+  const uint32_t rb = D * T::ESZ;
+  typename T::Stage st;
+  int32_t id[XPT], id_s = -1;       // pages of the next block to be loaded
+  uint32_t ok = 0, ok_next = 0;     // which of the stage's pieces are held (bit XPT: the scale)
+  auto pages = [&](uint32_t j) {
+    const uint32_t base = j * KB;
+#pragma unroll
+    for (int i = 0; i < XPT; ++i)
+      id[i] = base + xr[i] < reach ? paged_page(a.seqs, b, base + xr[i]) : -1;
+    if constexpr (T::kCodes)
+      id_s = t < 2 * KB && base + (t & 63) < reach ? paged_page(a.seqs, b, base + (t & 63)) : -1;
+  };
+  auto load = [&](uint32_t j) {
+    const uint32_t base = j * KB;
+    const char* kp = static_cast<const char*>(a.pool.k);
+    const char* vp = static_cast<const char*>(a.pool.v);
+    ok_next = 0;
+#pragma unroll
+    for (int i = 0; i < XPT; ++i) {
+      ok_next |= id[i] >= 0 ? 1u << i : 0u;
+      const uint64_t at =
+          pool_row(a.pool, a.seqs, max(id[i], 0), h,
+                   id[i] >= 0 ? paged_row(a.seqs, base + xr[i]) : 0u) * T::ESZ +
+          min(16u * xc[i], rb - 16);
+      st.k[i] = ldg128(kp + at);
+      st.v[i] = ldg128(vp + at);
+    }
+    if constexpr (T::kCodes) {
+      if (id_s >= 0) {
+        ok_next |= 1u << XPT;
+        st.scale = (t < KB ? a.pool.k_scale : a.pool.v_scale)[pool_scale(
+            a.pool, a.seqs, id_s, h, paged_row(a.seqs, base + (t & 63)))];
+      }
+    }
+  };
+  auto store = [&](uint32_t j) {   // what load(j) brought
+    char* const kl = sh.kv[j & 1];
+    char* const vl = kl + T::KBYTES;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < XPT; ++i) {
+      if (T::NX < NT && t >= T::NX) break;
+      u32x4 k = st.k[i], v = st.v[i];
+      const uint32_t r = xr[i], cc = xc[i];
+      if (16 * cc >= rb) k = u32x4{0, 0, 0, 0};   // (Q is zero there, K may be infinite)
+      if (!(ok >> i & 1)) v = u32x4{0, 0, 0, 0};
+      odd |= any_nonfinite<CT>(v);
+      if constexpr (T::kCodes) {
+        u32x2 w[8];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          w[x] = widen4<DT, CT>(k[x]);
+          w[4 + x] = widen4<DT, CT>(v[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          *reinterpret_cast<u32x4*>(kl + T::kaddr(r, 2 * cc + x)) =
+              u32x4{w[2 * x][0], w[2 * x][1], w[2 * x + 1][0], w[2 * x + 1][1]};
+          *reinterpret_cast<u32x4*>(vl + T::vaddr(r, 2 * cc + x)) =
+              u32x4{w[4 + 2 * x][0], w[4 + 2 * x][1], w[5 + 2 * x][0], w[5 + 2 * x][1]};
+        }
+      } else {
+        *reinterpret_cast<u32x4*>(kl + T::kaddr(r, cc)) = k;
+        *reinterpret_cast<u32x4*>(vl + T::vaddr(r, cc)) = v;
+      }
+      if (cc == 0 && (r & 15) == 0) sh.there[j & 1][r >> 4] = ok >> i & 1;
+    }
+    if constexpr (T::kCodes) {
+      if (t < 2 * KB)
+        (t < KB ? sh.ks : sh.vs)[j & 1][t & 63] = ok >> XPT & 1 ? st.scale : 0.0f;
+    }
+    if (odd && (j + 1) * KB > tile_min) sh.odd[j & 1] = j;   // (any of them: one value)
+  };
+
+  const uint32_t vlane = T::vaddr(4 * (lane >> 5) + ((lane & 15) >> 2),
+                                  (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) >> 3) +
+                         2 * (4 * (lane & 3) & 7);
+  const uint32_t klane = 128u * l32;
+  auto compute = [&](uint32_t j) {
+    const uint32_t base = j * KB;
+    if (base >= vis_max) return;   // uniform: nothing that the wave's rows see
+    const char* const kl = sh.kv[j & 1];
+    const char* const vl = kl + T::KBYTES;
+    f32x16 s[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+#pragma unroll
+    for (int ds = 0; ds < T::NDS; ++ds)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(
+            kl + (ds >> 2) * (KB * 128) + kt * 4096 + klane +
+            16 * ((2 * (ds & 3) + g) ^ T::kswz(l32)));
+        s[kt] = mfma32x32x16<DT>(kf, qf[ds], s[kt]);
+      }
+    // lane (row l32, g): accumulator r of half kt is position base + 32 kt + 8 (r / 4) + 4 g + r % 4
+    if constexpr (T::kCodes) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 ks = *reinterpret_cast<const f32x4*>(&sh.ks[j & 1][32 * kt + 8 * q + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[kt][4 * q + i] *= ks[i];
+        }
+    }
+    uint32_t there = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) there |= sh.there[j & 1][i] << i;
+    there = __builtin_amdgcn_readfirstlane(there);
+    const bool hides = base + KB > vis_min || there != 15;
+    const int lim = static_cast<int>(vis) - static_cast<int>(base) - 4 * g;
+    if (hides) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
+          if (at >= lim || !(there >> (at >> 4) & 1)) s[kt][i] = -INFINITY;
+        }
+    }
+    float mx[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      mx[q] = s[q >> 1][8 * (q & 1)];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx[q] = fmaxf(mx[q], s[q >> 1][8 * (q & 1) + i]);
+    }
+    const float top = pair_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * a.scale_log2;
+    float alpha = 1.0f;
+    bool moved = false;
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
+      const float mn = fmaxf(m, top);
+      alpha = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+      m = mn;
+      l *= alpha;
+      moved = true;
+    }
+    const float mu = m == -INFINITY ? 0.0f : m;
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[kt][i] = exp2_fast(__builtin_fmaf(s[kt][i], a.scale_log2, -mu));
+        (i & 1 ? l1 : l0) += s[kt][i];
+      }
+    l += l0 + l1;
+    if constexpr (T::kCodes) {
+      if constexpr (DT == kF16) {
+        // as in the rows' kernel: relative to the largest scale that the row has seen
+        float big = 0.0f;
+        if (hides) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
+              big = fmaxf(big, at < lim ? sh.vs[j & 1][at + 4 * g] : 0.0f);
+            }
+          big = pair_max(big);
+        } else {
+          big = wave_max(sh.vs[j & 1][lane]);
+        }
+        const int e = max(ev, big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000);
+        if (__builtin_amdgcn_ballot_w64(e > ev) != 0) {
+          alpha *= __builtin_ldexpf(1.0f, max(ev - e, -300));
+          ev = e;
+          moved = true;
+        }
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][32 * kt + 8 * q + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == kF16) vs[i] = __builtin_ldexpf(vs[i], ev < -500 ? 0 : -ev);
+            s[kt][4 * q + i] *= vs[i];
+          }
+        }
+      if (hides) {   // (a hidden token's scale may be NaN)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * kt + 8 * (i >> 2) + (i & 3) >= lim) s[kt][i] = 0.0f;
+      }
+    }
+    if (moved) {
+#pragma unroll
+      for (int i = 0; i < T::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc[i][x] *= alpha;
+    }
+    if (hides && __builtin_amdgcn_readfirstlane(sh.odd[j & 1]) == j && vis_min < reach) {
+      // NaN or infinities among values that some rows do not see (0 * NaN is NaN): this block on
+      // the vector ALUs, each row over what it sees
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {
+#pragma unroll 1
+        for (int gk = 0; gk < 2; ++gk) {
+          const float pk = __shfl(s[0][0], l32 + 32 * gk);
+          const uint32_t r = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * gk + (i & 3);
+          if (base + r < vis) {
+#pragma unroll
+            for (int dt = 0; dt < T::NDT; ++dt)
+#pragma unroll
+              for (int x = 0; x < 16; ++x) {
+                const uint32_t d = 32 * dt + 8 * (x >> 2) + 4 * g + (x & 3);
+                const uint16_t v =
+                    *reinterpret_cast<const uint16_t*>(vl + T::vaddr(r, d >> 3) + 2 * (d & 7));
+                acc[dt][x] = __builtin_fmaf(pk, u16_to_f32<DT>(v), acc[dt][x]);
+              }
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 31; ++x) s[x >> 4][x & 15] = s[(x + 1) >> 4][(x + 1) & 15];
+      }
+      return;
+    }
+#pragma unroll
+    for (int sp = 0; sp < 4; ++sp) {
+      const int o = 8 * (sp & 1);
+      const f32x16& p = s[sp >> 1];
+      const u32x4 pf = {pack2h<DT>(p[o], p[o + 1]), pack2h<DT>(p[o + 2], p[o + 3]),
+                        pack2h<DT>(p[o + 4], p[o + 5]), pack2h<DT>(p[o + 6], p[o + 7])};
+#pragma unroll
+      for (int dt = 0; dt < T::NDT; ++dt) {
+        // columns 32 dt on: chunk bits 2 and up, which the swizzle's bit 2 meets by XOR
+        const uint32_t va = vlane ^ (dt << 6);
+        const u32x2 lo = lds::read_tr16(vl + va + 16 * T::RB * sp);
+        const u32x2 hi = lds::read_tr16(vl + va + 16 * T::RB * sp + 8 * T::RB);
+        acc[dt] = mfma32x32x16<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, acc[dt]);
+      }
+    }
+  };
+
+  if (j0 < j1) {
+    pages(j0);
+    load(j0);
+    ok = ok_next;
+    if (j0 + 1 < j1) pages(j0 + 1);
+    __syncthreads();   // (sh.odd)
+    store(j0);
+    if (j0 + 1 < j1) {
+      load(j0 + 1);
+      ok = ok_next;
+    }
+    if (j0 + 2 < j1) pages(j0 + 2);
+    for (uint32_t j = j0; j < j1; ++j) {
+      // block j is whole in LDS, and every wave is done with block j - 1, whose half block
+      // j + 1 takes
+      __syncthreads();
+      if (j + 1 < j1) store(j + 1);
+      if (j + 2 < j1) {
+        load(j + 2);
+        ok = ok_next;
+      }
+      if (j + 3 < j1) pages(j + 3);
+      compute(j);
+    }
+  }
+  if (!live_wave) return;
+  l = pair_sum(l);
+  if constexpr (T::kCodes && DT == kF16) {
+#pragma unroll
+    for (int i = 0; i < T::NDT; ++i)
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        acc[i][x] = ev < -500 ? 0.0f : __builtin_ldexpf(acc[i][x], ev);
+  }
+  if (!live_row) return;
+  const uint64_t at = (c.first + qi) * static_cast<uint64_t>(a.nh) + hq;
+  if (whole) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < T::NDT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t d = 32 * i + 8 * q + 4 * g;
+        float f[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[x] = l == 0.0f ? 0.0f : acc[i][4 * q + x] * inv;
+        if (d < D)
+          *reinterpret_cast<u32x2*>(a.o + at * D + d) =
+              u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
+      }
+  } else {
+    float* const rec_ =
+        a.chunk_ws +
+        (static_cast<uint64_t>(part) * a.seqs.total_q * a.nh + at) * rec(HD);
+#pragma unroll
+    for (int i = 0; i < T::NDT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(rec_ + 32 * i + 8 * q + 4 * g) =
+            f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+    if (g == 0) {
+      rec_[HD] = l;
+      rec_[HD + 1] = m;
+    }
+  }
+}
+
+// Merge a chunk tile's parts: one workgroup per token, HD / 4 lanes per row.
+template <int DT, int HD>
+__global__ void __launch_bounds__(256)
+attn_paged_chunk_merge(AttnArgs a) {
+  using namespace chunk;
+  constexpr int LPR = HD / 4, RPB = 256 / LPR;
+  const uint32_t lane = threadIdx.x & 63u, token = blockIdx.x;
+  uint32_t le = 0;
+  for (uint32_t j0 = 0; j0 < a.seqs.batch; j0 += 64) {
+    const uint32_t j = j0 + lane;
+    le += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
+        j < a.seqs.batch && paged_clamp(a.seqs.q_start[j], a.seqs.total_q) <= token));
+  }
+  if (le == 0) return;
+  const PagedChunk c = paged_chunk(a.seqs, le - 1);
+  if (token < c.first || token - c.first >= c.n || c.n * a.group <= a.split_rows) return;
+  const int d = 4 * (threadIdx.x % LPR);
+  for (uint32_t hq = threadIdx.x / LPR; hq < a.nh; hq += RPB) {
+    const uint32_t row = (token - c.first) * a.group + hq % a.group;
+    const uint32_t reach = tile_reach(a, c, row / TR);
+    const uint32_t per = part_blocks(reach, a.parts), nb = (reach + KB - 1) / KB;
+    if (per >= nb) continue;
+    const uint32_t np = (nb + per - 1) / per;
+    const uint64_t step = static_cast<uint64_t>(a.seqs.total_q) * a.nh * rec(HD);
+    const float* r = a.chunk_ws + (static_cast<uint64_t>(token) * a.nh + hq) * rec(HD);
+    float M = -INFINITY;
+    for (uint32_t p = 0; p < np; ++p) M = fmaxf(M, r[p * step + HD + 1]);
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t p = 0; p < np; ++p) {
+      const float lp = r[p * step + HD], mp = r[p * step + HD + 1];
+      if (lp == 0.0f) continue;   // a part that the row sees nothing of
+      const float w = mp == -INFINITY ? 0.0f : exp2_fast(mp - M);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(r + p * step + d);
+      l = __builtin_fmaf(w, lp, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, x[i], o[i]);
+    }
+    if (d < static_cast<int>(a.pool.head_dim)) {
+      float f[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = l == 0.0f ? 0.0f : o[i] / l;
+      *reinterpret_cast<u32x2*>(a.o + (static_cast<uint64_t>(token) * a.nh + hq) * a.pool.head_dim +
+                                d) = u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
+    }
   }
 }
 

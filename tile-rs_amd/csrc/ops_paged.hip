@@ -100,32 +100,74 @@ void by_float(th_dtype d, F&& f) {
 
 // ---- attention ---------------------------------------------------------------------------
 
-// Runs that the units are dealt to, at most: two workgroups per CU of a whole MI355X.
-constexpr uint32_t kMaxRuns = 512;
-
 uint32_t head_width(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-// At least the units of any lengths that the structs allow.
-uint64_t most_units(const th::PagedSeqs& s, uint32_t nkv, uint32_t group) {
-  const uint64_t tiles =
-      static_cast<uint64_t>(s.total_q) * group / th::pgd::rows::TR + s.batch;
-  const uint64_t per = s.cap / th::pgd::rows::UNIT + 1;
-  const uint64_t cap = uint64_t{1} << 40;
-  return std::min(cap, std::min(cap, tiles * nkv) * per);
-}
+// How a call is split over its kernels, from what the host knows: the structs' sizes.
+struct AttnPlan {
+  uint32_t runs = 0;         // workgroups of the rows' kernel (0: not launched)
+  uint32_t split_rows = 0;   // sequences of more rows go to the chunks' kernel
+  uint64_t items = 0;        // (tile, head) items of the chunks' kernel, at most (0: not launched)
+  uint32_t parts = 1;
+  size_t rows_bytes = 0, chunk_bytes = 0;
+};
 
-size_t paged_room(const th::PagedSeqs& s, uint32_t nkv, uint32_t group, uint32_t head_dim) {
-  const uint64_t runs = std::min<uint64_t>(kMaxRuns, most_units(s, nkv, group));
-  return runs * 2 * th::pgd::rows::rec(static_cast<int>(head_width(head_dim))) * sizeof(float);
+// Runs that the rows' units are dealt to: two workgroups per CU.  CUs of a whole MI355X, not of
+// the current device, so that the workspace's size does not depend on it.
+constexpr uint32_t kCus = 256, kMaxRuns = 2 * kCus;
+// Rows up to which a sequence stays with the rows' kernel.
+constexpr uint32_t kSplitRows = 64;
+
+AttnPlan attn_plan(const th::PagedSeqs& s, uint32_t nkv, uint32_t group, uint32_t head_dim) {
+  AttnPlan p;
+  const uint32_t hd = head_width(head_dim);
+  const uint64_t rows = static_cast<uint64_t>(s.total_q) * group;
+  // a token per sequence: all of them steps, most likely
+  const bool chunks = hd <= 128 && rows > kSplitRows && s.total_q > s.batch;
+  p.split_rows = !chunks ? 0xffffffffu : s.batch == 1 ? 0u : kSplitRows;
+  if (p.split_rows != 0) {
+    // at least the units of any lengths that the structs allow
+    const uint64_t tiles = rows / th::pgd::rows::TR + s.batch;
+    const uint64_t cap = uint64_t{1} << 40;
+    const uint64_t units =
+        std::min(cap, std::min(cap, tiles * nkv) * (s.cap / th::pgd::rows::UNIT + 1));
+    p.runs = static_cast<uint32_t>(std::min<uint64_t>(kMaxRuns, units));
+    p.rows_bytes =
+        static_cast<size_t>(p.runs) * 2 * th::pgd::rows::rec(static_cast<int>(hd)) * sizeof(float);
+  }
+  if (chunks) {
+    const uint64_t some = rows / (p.split_rows + 1);   // sequences of more than split_rows rows
+    const uint64_t tiles = rows / th::pgd::chunk::TR + std::min<uint64_t>(s.batch, some);
+    p.items = std::max<uint64_t>(1, tiles) * nkv;
+    const uint32_t most = std::max(1u, s.cap / th::pgd::chunk::KB / th::pgd::chunk::kLeast);
+    if (p.items < kCus)
+      p.parts = static_cast<uint32_t>(
+          std::min<uint64_t>(std::min(16u, most), (kCus + p.items - 1) / p.items));
+    if (p.parts > 1)
+      p.chunk_bytes = static_cast<size_t>(p.parts) * s.total_q * nkv * group *
+                      th::pgd::chunk::rec(static_cast<int>(hd)) * sizeof(float);
+  }
+  return p;
 }
 
 template <int DT, int CT, int HD>
-void attn_paged_go(const th::pgd::AttnArgs& a, uint32_t runs, hipStream_t s) {
-  hipLaunchKernelGGL((th::pgd::attn_paged_rows<DT, CT, HD>), dim3(runs), dim3(th::pgd::rows::NT), 0,
-                     s, a);
-  if (runs > 1)
-    hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, CT, HD>), dim3(runs - 1), dim3(256), 0, s, a,
-                       runs);
+void attn_paged_go(const th::pgd::AttnArgs& a, const AttnPlan& p, hipStream_t s) {
+  if (p.runs) {
+    hipLaunchKernelGGL((th::pgd::attn_paged_rows<DT, CT, HD>), dim3(p.runs),
+                       dim3(th::pgd::rows::NT), 0, s, a);
+    if (p.runs > 1)
+      hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, CT, HD>), dim3(p.runs - 1), dim3(256), 0,
+                         s, a, p.runs);
+  }
+  if constexpr (HD <= 128) {
+    if (p.items) {
+      hipLaunchKernelGGL((th::pgd::attn_paged_chunk<DT, CT, HD>),
+                         dim3(static_cast<uint32_t>(p.items * p.parts)), dim3(th::pgd::chunk::NT),
+                         0, s, a);
+      if (p.parts > 1)
+        hipLaunchKernelGGL((th::pgd::attn_paged_chunk_merge<DT, HD>), dim3(a.seqs.total_q),
+                           dim3(256), 0, s, a);
+    }
+  }
 }
 
 }  // namespace
@@ -197,7 +239,8 @@ size_t th_attention_paged_workspace_size(const th_kv_pages* pages, const th_kv_b
       num_heads == 0 || num_heads % pool.nkv != 0)
     return 0;   // (th_attention_paged refuses the same arguments)
   if (sq.batch == 0 || sq.total_q == 0) return 0;
-  return paged_room(sq, pool.nkv, num_heads / pool.nkv, pool.head_dim);
+  const AttnPlan p = attn_plan(sq, pool.nkv, num_heads / pool.nkv, pool.head_dim);
+  return p.rows_bytes + p.chunk_bytes;
 }
 
 int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batch* seqs, void* o,
@@ -231,7 +274,10 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
   a.nh = num_heads;
   a.group = num_heads / nkv;
   a.scale_log2 = th::kLog2e / std::sqrt(static_cast<float>(D));
-  const size_t need = paged_room(a.seqs, nkv, a.group, D);
+  const AttnPlan plan = attn_plan(a.seqs, nkv, a.group, D);
+  if (plan.items * plan.parts > 0x7fffffffu)
+    return fail(TH_KERNEL_ERROR, "attention_paged: grid too large");
+  const size_t need = plan.rows_bytes + plan.chunk_bytes;
   th::ScratchHold hold;
   if (workspace) {
     if (workspace_bytes < need)
@@ -241,19 +287,20 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
     if (!aligned16(workspace))
       return fail(TH_KERNEL_ERROR, "attention_paged: workspace must be 16-byte aligned");
   } else {
-    if (stream_capturing(as_stream(s)))
+    if (need && stream_capturing(as_stream(s)))
       return fail(TH_MEMORY_ERROR,
                   "attention_paged: a stream that is being captured needs a workspace");
-    TH_TRY(th::stream_scratch(as_stream(s), need, &workspace, &hold));
+    if (need) TH_TRY(th::stream_scratch(as_stream(s), need, &workspace, &hold));
   }
   a.ws = static_cast<float*>(workspace);
-  const uint32_t runs = static_cast<uint32_t>(std::min<uint64_t>(
-      std::min(kMaxRuns, 2 * current_cu_count()), most_units(a.seqs, nkv, a.group)));
+  a.chunk_ws = a.ws + plan.rows_bytes / sizeof(float);
+  a.split_rows = plan.split_rows;
+  a.parts = plan.parts;
   auto go = [&](auto dt, auto ct) {
     switch (head_width(D)) {
-      case 64: attn_paged_go<dt.value, ct.value, 64>(a, runs, as_stream(s)); break;
-      case 128: attn_paged_go<dt.value, ct.value, 128>(a, runs, as_stream(s)); break;
-      default: attn_paged_go<dt.value, ct.value, 256>(a, runs, as_stream(s)); break;
+      case 64: attn_paged_go<dt.value, ct.value, 64>(a, plan, as_stream(s)); break;
+      case 128: attn_paged_go<dt.value, ct.value, 128>(a, plan, as_stream(s)); break;
+      default: attn_paged_go<dt.value, ct.value, 256>(a, plan, as_stream(s)); break;
     }
   };
   auto cache = [&](auto dt) {
