@@ -62,6 +62,30 @@ __device__ __forceinline__ u32x2 widen4(uint32_t w) {
   return out;
 }
 
+// paged_page with a scalar load, for a sequence and position that the whole wave shares.  (The
+// table does not change while a call runs.)
+__device__ __forceinline__ int32_t wave_page(const PagedSeqs& s, uint32_t b, uint32_t pos) {
+  typedef __attribute__((address_space(4))) const int32_t* scalar_ptr;
+  b = __builtin_amdgcn_readfirstlane(b);
+  pos = __builtin_amdgcn_readfirstlane(pos);
+  if (pos >= s.cap) return -1;
+  const uint64_t at = static_cast<uint64_t>(b) * s.max_pages + (pos >> s.shift);
+  const int32_t id = *(scalar_ptr)(reinterpret_cast<uintptr_t>(s.table + at));
+  return id >= 0 && static_cast<uint32_t>(id) < s.num_pages ? id : -1;
+}
+
+// 16 bytes at `off` of the `bytes` bytes at p, zeros past them (the buffer's range check): p and
+// bytes are the wave's, off is the lane's.
+template <bool NT>
+__device__ __forceinline__ u32x4 load_within(const void* p, uint32_t bytes, uint32_t off) {
+  const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes),
+                                                   0x00020000);
+  return __builtin_bit_cast(
+      u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(off), 0, NT ? 2 : 0));
+}
+// An offset that is past every range.
+constexpr uint32_t kPast = 0x7ffffff0u;
+
 // Whether a NaN or an infinity is among the 16 bytes.
 template <int CT>
 __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
@@ -78,7 +102,7 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
   return bad;
 }
 
-// ---- the rows' kernel: tiles of 16 rows, the positions split over the chip ---------------
+// ---- the rows' kernel: tiles of 16 or 32 rows, the positions split over the chip -----------
 //
 // For steps of one or a few tokens, which are bound by the cache's bytes.  The unit of work is
 // UNIT positions of one (sequence, tile, kv head); the units of the whole batch, in that order,
@@ -88,18 +112,18 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
 // (slot 2 w) and one that begins its tile (slot 2 w + 1).
 //
 // Within a workgroup each wave has 32 of the unit's positions to itself, with running maximum
-// and sum of its own, so nothing waits for a barrier until the run's end.  Per 32 positions:
+// and sum of its own, so nothing waits for a barrier until the run's end.  Per 32 positions and
+// 16 rows:
 //   S^T (32 x 16) = K . Q^T     16x16x32 MFMA; K fragments come straight from global memory
 //   O^T (D x 16) += V^T . P^T   P^T is S^T's accumulator layout, its 16 positions' tiles
 //                               interleaved as the k index; V goes through the wave's own LDS,
 //                               whose transposing read gives V^T in the same order
-// The next 32 positions' K and V are in flight meanwhile.  The maximum is only moved where a
-// score passes it by 8 (2^8 of headroom in the 16-bit probabilities).
+// The next 32 positions are loaded as soon as K is multiplied and V is in LDS.  The maximum is
+// only moved where a score passes it by 8 (2^8 of headroom in the 16-bit probabilities).
 namespace rows {
 constexpr int NT = 256;
-constexpr int TR = 16;       // rows of a tile
 constexpr int UNIT = 128;    // positions of a unit: 32 for each wave
-constexpr int rec(int hd) { return TR * (hd + 2); }   // floats of a part: O, then m, then l
+constexpr int rec(int hd, int tr) { return tr * (hd + 2); }   // floats of a part: O, then m, l
 }  // namespace rows
 
 struct AttnArgs {
@@ -111,85 +135,118 @@ struct AttnArgs {
   uint64_t q_stride;
   float scale_log2;
   uint32_t nh, group;
+  uint32_t tile_rows;    // of the rows' kernel: 16 or 32
   uint32_t split_rows;   // sequences of more rows are the chunk kernel's, the others the rows'
+  uint32_t runs;         // workgroups of the rows' kernel
   uint32_t parts;        // parts that a chunk tile's positions are cut into, at most
   float* chunk_ws;       // the chunk kernel's sums: [parts][total_q * nh] records
 };
-
-// Work of one sequence: tiles of TR rows, and units of UNIT positions (one at least, so that rows
-// without any position are written too).
-struct SeqWork {
-  uint32_t tiles, units;
-};
-__device__ __forceinline__ SeqWork rows_work(const AttnArgs& a, const PagedChunk& c) {
-  SeqWork w;
-  const uint32_t r = c.n * a.group;   // the host keeps total_q * num_heads below 2^31
-  w.tiles = r <= a.split_rows ? (r + rows::TR - 1) / rows::TR : 0u;
-  const uint32_t u = c.held / rows::UNIT + (c.held % rows::UNIT != 0);
-  w.units = u == 0 ? 1u : u;
-  return w;
-}
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
   const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), d);
   const uint32_t hi = __shfl_up(static_cast<uint32_t>(v >> 32), d);
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
+__device__ __forceinline__ uint32_t read_lane(uint32_t v, int l) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+}
 __device__ __forceinline__ uint64_t read_lane64(uint64_t v, int l) {
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
-  return static_cast<uint64_t>(hi) << 32 | lo;
+  return static_cast<uint64_t>(read_lane(static_cast<uint32_t>(v >> 32), l)) << 32 |
+         read_lane(static_cast<uint32_t>(v), l);
 }
 
-// Units of all sequences; and the sequence that holds unit u, with the units before it.  Each
-// wave scans on its own, 64 sequences at a time.  (Units of a batch stay far below 2^63: under
-// 2^31 rows of 2^25 units and 2^32 heads would not fit any memory.)
-struct Where {
-  uint32_t b;
-  uint64_t before;
+// The rows' units of 64 sequences, one per lane.  A sequence has tiles x heads x (blocks of its
+// positions, one at least, so that rows without any position are written too) units.  (All of a
+// batch's stay far below 2^63: 2^31 rows, 2^25 blocks.)
+struct SeqGroup {
+  PagedChunk c;
+  uint32_t tiles, blocks;
+  uint64_t units, upto;   // of this lane's sequence, and of all up to it
 };
-template <class F>
-__device__ __forceinline__ uint64_t scan_units(const AttnArgs& a, F&& visit) {
+__device__ __forceinline__ SeqGroup seq_group(const AttnArgs& a, uint32_t b0, uint64_t before) {
   const uint32_t lane = threadIdx.x & 63u;
-  uint64_t sum = 0;
-  for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
-    uint64_t u = 0;
-    if (b0 + lane < a.seqs.batch) {
-      const SeqWork w = rows_work(a, paged_chunk(a.seqs, b0 + lane));
-      u = static_cast<uint64_t>(w.tiles) * w.units * a.pool.nkv;
-    }
-    uint64_t inc = u;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint64_t x = shfl_up64(inc, d);
-      if (lane >= static_cast<uint32_t>(d)) inc += x;
-    }
-    visit(b0, sum, u, inc);
-    sum += read_lane64(inc, 63);
+  SeqGroup g{};
+  if (b0 + lane < a.seqs.batch) {
+    g.c = paged_chunk(a.seqs, b0 + lane);
+    const uint32_t r = g.c.n * a.group;   // the host keeps total_q * num_heads below 2^31
+    g.tiles = r <= a.split_rows ? (r + a.tile_rows - 1) / a.tile_rows : 0u;
+    g.blocks = max(1u, g.c.held / rows::UNIT + (g.c.held % rows::UNIT != 0));
+    g.units = static_cast<uint64_t>(g.tiles) * g.blocks * a.pool.nkv;
   }
-  return sum;
+  g.upto = g.units;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint64_t x = shfl_up64(g.upto, d);
+    if (lane >= static_cast<uint32_t>(d)) g.upto += x;
+  }
+  g.upto += before;
+  return g;
 }
-__device__ __forceinline__ Where find_unit(const AttnArgs& a, uint64_t target) {
-  Where w{a.seqs.batch, 0};
-  scan_units(a, [&](uint32_t b0, uint64_t sum, uint64_t u, uint64_t inc) {
-    const uint64_t in = __builtin_amdgcn_ballot_w64(sum + inc - u <= target && target < sum + inc);
-    if (in != 0) {   // exactly one lane
-      const int l = __builtin_ctzll(in);
-      w.b = b0 + l;
-      w.before = sum + read_lane64(inc, l) - read_lane64(u, l);
+
+// A place among the units: the sequence that holds unit u.  Every wave finds it on its own.
+struct Place {
+  SeqGroup g;      // of the 64 sequences from b0 on
+  uint32_t b0;
+  int l;           // the sequence's lane
+  uint64_t units;  // of the whole batch
+
+  __device__ __forceinline__ explicit Place(const AttnArgs& a) : g(seq_group(a, 0, 0)), b0(0), l(0) {
+    units = read_lane64(g.upto, 63);
+    if (a.seqs.batch > 64) {
+      SeqGroup x = g;
+      for (uint32_t i = 64; i < a.seqs.batch; i += 64) {
+        x = seq_group(a, i, units);
+        units = read_lane64(x.upto, 63);
+      }
     }
-  });
-  return w;
-}
+  }
+  // From the present group on; false if no sequence holds u (lengths that change under the call).
+  __device__ __forceinline__ bool find(const AttnArgs& a, uint64_t u) {
+    while (true) {
+      const uint64_t in = __builtin_amdgcn_ballot_w64(g.upto - g.units <= u && u < g.upto);
+      if (in != 0) {   // exactly one lane
+        l = __builtin_ctzll(in);
+        return true;
+      }
+      b0 += 64;
+      if (b0 >= a.seqs.batch) return false;
+      g = seq_group(a, b0, read_lane64(g.upto, 63));
+    }
+  }
+  __device__ __forceinline__ PagedChunk chunk() const {
+    PagedChunk c;
+    c.first = read_lane(g.c.first, l);
+    c.n = read_lane(g.c.n, l);
+    c.base = static_cast<int32_t>(read_lane(static_cast<uint32_t>(g.c.base), l));
+    c.held = read_lane(g.c.held, l);
+    return c;
+  }
+};
 // First unit of run w of n.
 __device__ __forceinline__ uint64_t run_start(uint64_t units, uint32_t w, uint32_t n) {
   return units / n * w + min(static_cast<uint64_t>(w), units % n);
 }
 
-template <int DT, int CT, int HD>
+// Eight values of O from their weighted sum and the weights' sum.
+template <int DT>
+__device__ __forceinline__ void write_row(const AttnArgs& a, const PagedChunk& c, uint32_t h,
+                                          uint32_t row, int c8, const float (&o)[8], float l) {
+  const uint64_t tok = c.first + row / a.group;
+  const uint32_t hq = h * a.group + row % a.group;
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = l == 0.0f ? 0.0f : o[j] / l;
+  *reinterpret_cast<u32x4*>(a.o + (tok * a.nh + hq) * a.pool.head_dim + c8) =
+      u32x4{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3]), pack2h<DT>(f[4], f[5]),
+            pack2h<DT>(f[6], f[7])};
+}
+
+template <int DT, int CT, int HD, int MT>
 struct RowsTile {
   static constexpr bool kCodes = cache_codes<CT>();
+  static constexpr bool kExps = kCodes && DT == kF16;   // scales enter relative to 2^ev
   static constexpr int ESZ = cache_size<CT>();
+  static constexpr int TR = 16 * MT;
   static constexpr int NS = HD / 32;             // K fragments (32 values deep) of a position
   static constexpr int NC = HD / 16;             // 16-wide column tiles of O
   static constexpr int KL = 2 * HD * ESZ / 64;   // 16-byte K loads per lane: 2 tiles x HD/4 values
@@ -198,14 +255,19 @@ struct RowsTile {
   static_assert(VL >= 2, "a V load lies in one half of the 32 rows");
   static constexpr int ORS = HD + 4;             // row stride of the merge arena (floats)
   static constexpr int VB = 32 * HD * 2;         // V in LDS, bytes per wave
-  static constexpr int OB = rows::TR * ORS * 4;  // O at the end, bytes per wave
+  static constexpr int OB = TR * ORS * 4;        // O at the end, bytes per wave
   static constexpr int WB = VB > OB ? VB : OB;
 
-  // What is in flight for 32 positions.
+  // 32 positions on their way.
   struct Stage {
     u32x4 k[KL], v[VL];
     f32x4 ks[2], vs[2];
-    bool there[2];   // the pages of positions 0-15 and 16-31 exist
+    int32_t page[2];   // of positions 0-15 and 16-31, or -1
+  };
+  struct Sums {
+    f32x4 acc[MT][NC];
+    float m[MT], l[MT];   // m: the row's (all its lanes); l: this lane's positions
+    int ev[MT];
   };
 
   // 16-byte chunk c of V row r (32 rows of HD 16-bit values) in LDS: the four rows of a
@@ -215,51 +277,53 @@ struct RowsTile {
     return r * (HD * 2) + ((c ^ x) << 4);
   }
 
-  static __device__ __forceinline__ void load(const AttnArgs& a, uint32_t b, uint32_t h,
-                                              uint32_t base, uint32_t held, Stage& st) {
-    const PagedPool& p = a.pool;
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    uint64_t at[2], sc[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      // pages hold whole groups of 16 positions
-      const uint32_t pos = base + 16 * t;
-      const int32_t page = pos < held ? paged_page(a.seqs, b, pos) : -1;
-      st.there[t] = page >= 0;
-      const int32_t id = page >= 0 ? page : 0;   // num_pages >= 1; what is loaded is not used
-      const uint32_t row = page >= 0 ? paged_row(a.seqs, pos) : 0u;
-      at[t] = pool_row(p, a.seqs, id, h, row) * ESZ;
-      sc[t] = pool_scale(p, a.seqs, id, h, row);
-    }
-    const uint32_t rb = p.head_dim * ESZ;   // bytes of a row
-    const char* kp = static_cast<const char*>(p.k);
-    const char* vp = static_cast<const char*>(p.v);
+  // Pages hold whole groups of 16 positions.
+  static __device__ __forceinline__ void pages(const AttnArgs& a, uint32_t b, uint32_t base,
+                                               uint32_t held, int32_t (&page)[2]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
+      page[t] = base + 16 * t < held ? wave_page(a.seqs, b, base + 16 * t) : -1;
+  }
+
+  // Rows of missing pages and from `end` on are loaded as zeros.
+  static __device__ __forceinline__ void load(const AttnArgs& a, uint32_t h, uint32_t base,
+                                              uint32_t end, const int32_t (&page)[2], Stage& st) {
+    const PagedPool& p = a.pool;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const uint32_t rb = p.head_dim * ESZ;   // bytes of a row
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t pos = base + 16 * t;
+      const uint32_t n = page[t] >= 0 && pos < end ? min(16u, end - pos) : 0u;
+      const int32_t id = max(page[t], 0);
+      const uint32_t row = paged_row(a.seqs, pos);
+      st.page[t] = page[t];
+      const uint64_t at = pool_row(p, a.seqs, id, h, row) * ESZ;
+      const char* const kp = static_cast<const char*>(p.k) + at;
+      const char* const vp = static_cast<const char*>(p.v) + at;
 #pragma unroll
       for (int i = 0; i < KL / 2; ++i) {
         const uint32_t c = 64 * i + 16 * g;
-        u32x4& k = st.k[t * (KL / 2) + i];
-        k = ldg128_nt(kp + at[t] + l16 * rb + min(c, rb - 16));
-        if (c >= rb) k = u32x4{0, 0, 0, 0};   // (Q is zero there, K may be infinite)
+        st.k[t * (KL / 2) + i] = load_within<true>(kp, n * rb, c < rb ? l16 * rb + c : kPast);
       }
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const uint32_t r = i * (32 / VL) + lane / VROW;   // rows 0-15 in the first half of loads
-      const uint32_t c = min(16u * (lane % VROW), rb - 16);
-      st.v[i] = ldg128_nt(vp + at[2 * i / VL] + (r & 15) * rb + c);
-    }
-    if constexpr (kCodes) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        st.ks[t] = *reinterpret_cast<const f32x4*>(p.k_scale + sc[t] + 4 * g);
-        st.vs[t] = *reinterpret_cast<const f32x4*>(p.v_scale + sc[t] + 4 * g);
+      for (int i = 0; i < VL / 2; ++i) {
+        const uint32_t r = i * (32 / VL) + lane / VROW, c = 16u * (lane % VROW);
+        st.v[t * (VL / 2) + i] = load_within<true>(vp, n * rb, c < rb ? r * rb + c : kPast);
+      }
+      if constexpr (kCodes) {
+        const uint64_t sc = pool_scale(p, a.seqs, id, h, row);
+        st.ks[t] = __builtin_bit_cast(f32x4, load_within<false>(p.k_scale + sc, n * 4, 16 * g));
+        st.vs[t] = __builtin_bit_cast(f32x4, load_within<false>(p.v_scale + sc, n * 4, 16 * g));
       }
     }
   }
 
   // K fragment s of tile t, 8 values per lane.  16 bits: columns 32 s + 8 g; codes: a lane's 16
   // bytes are columns 64 (s / 2) + 16 g .. + 15, fragment s its half s % 2 (Q is read alike).
+  static __device__ __forceinline__ uint32_t qcol(int s, int g) {
+    return kCodes ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g;
+  }
   static __device__ __forceinline__ u32x4 kfrag(const Stage& st, int t, int s) {
     if constexpr (kCodes) {
       const u32x4 w = st.k[t * (KL / 2) + s / 2];
@@ -269,22 +333,18 @@ struct RowsTile {
       return st.k[t * (KL / 2) + s];
     }
   }
-  static __device__ __forceinline__ uint32_t qcol(int s, int g) {
-    return kCodes ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g;
-  }
 
-  // V of the stage into LDS, rows from `live` on and rows of missing pages as zeros.
-  static __device__ __forceinline__ void put_v(const Stage& st, char* lds, uint32_t live) {
+  // V of the stage into LDS.
+  static __device__ __forceinline__ void put_v(const Stage& st, char* lds) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       const uint32_t r = i * (32 / VL) + lane / VROW, c = lane % VROW;
-      u32x4 w = st.v[i];
-      if (r >= live || !st.there[2 * i / VL]) w = u32x4{0, 0, 0, 0};
+      const u32x4 w = st.v[i];
       if constexpr (kCodes) {
         const u32x2 a = widen4<DT, CT>(w[0]), b = widen4<DT, CT>(w[1]);
-        const u32x2 d = widen4<DT, CT>(w[2]), e = widen4<DT, CT>(w[3]);
         *reinterpret_cast<u32x4*>(lds + vaddr(r, 2 * c)) = u32x4{a[0], a[1], b[0], b[1]};
+        const u32x2 d = widen4<DT, CT>(w[2]), e = widen4<DT, CT>(w[3]);
         *reinterpret_cast<u32x4*>(lds + vaddr(r, 2 * c + 1)) = u32x4{d[0], d[1], e[0], e[1]};
       } else {
         *reinterpret_cast<u32x4*>(lds + vaddr(r, c)) = w;
@@ -299,7 +359,7 @@ struct RowsTile {
   }
 
   // acc += V^T . P^T, V from LDS.
-  static __device__ __forceinline__ void pv(const char* lds, u32x4 pf, f32x4 (&acc)[NC]) {
+  static __device__ __forceinline__ void pv(const char* lds, const u32x4 (&pf)[MT], Sums& y) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t r = 4 * g + (l16 >> 2);
 #pragma unroll
@@ -308,321 +368,362 @@ struct RowsTile {
       const uint32_t ch = 2 * c + ((l16 & 3) >> 1), in = 8 * (l16 & 1);
       const u32x2 lo = lds::read_tr16(lds + vaddr(r, ch) + in);
       const u32x2 hi = lds::read_tr16(lds + vaddr(16 + r, ch) + in);
-      acc[c] = mfma16x16x32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, acc[c]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        y.acc[i][c] = mfma16x16x32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[i], y.acc[i][c]);
     }
   }
 
-  // Units [k0, k1) of tile `tile` of (b, h): the wave's share, then the workgroup's sum.
+  // The same for one tile on the vector ALUs, each row over the first `see` positions.  (Rare, so
+  // it is kept small: what it needs in registers is taken from all that comes before.)
+  static __device__ __forceinline__ void pv_seen(const char* lds, u32x4 pf, uint32_t see,
+                                                 f32x4 (&acc)[NC]) {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll 1
+      for (int gk = 0; gk < 4; ++gk) {
+        const uint32_t w = __shfl(pf[0], l16 + 16 * gk);
+        const float pk = u16_to_f32<DT>(static_cast<uint16_t>(w >> (16 * (i & 1))));
+        const uint32_t r = 16 * (i >> 2) + 4 * gk + (i & 3);
+        if (r < see) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            uint32_t dg = 4 * g;
+            asm volatile("" : "+v"(dg) : : "memory");
+            const uint32_t d = 16 * c + dg;
+            const u32x2 x = *reinterpret_cast<const u32x2*>(lds + vaddr(r, d >> 3) + 2 * (d & 7));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[c][j] = __builtin_fmaf(
+                  pk, u16_to_f32<DT>(static_cast<uint16_t>(x[j >> 1] >> (16 * (j & 1)))),
+                  acc[c][j]);
+          }
+        }
+      }
+      if (i & 1) pf = u32x4{pf[1], pf[2], pf[3], pf[0]};
+    }
+  }
+
+  // Blocks [k0, k1) of tile `tile` of (b, h): the wave's share, then the workgroup's sum.
   // part: where the sums go, or null: O.
   static __device__ __forceinline__ void run(const AttnArgs& a, const PagedChunk& c, uint32_t b,
                                              uint32_t h, uint32_t tile, uint32_t k0, uint32_t k1,
-                                             float* part, char* arena) {
+                                             float* part, char* arena, u32x4* q_lds) {
     const int t = threadIdx.x, lane = t & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t D = a.pool.head_dim, G = a.group;
     const uint32_t nrows = c.n * G;
-    const uint32_t row = tile * rows::TR + l16;
-    const bool live_row = row < nrows;
-    const uint32_t qi = row / G, hq = h * G + row % G;
-    const uint32_t vis = live_row ? paged_visible(c, qi) : 0u;
     // the tile's first and last rows bound what its rows see
-    const uint32_t r0 = tile * rows::TR, r1 = min(nrows, r0 + rows::TR) - 1;
+    const uint32_t r0 = tile * TR, r1 = min(nrows, r0 + TR) - 1;
     const uint32_t vis_min = __builtin_amdgcn_readfirstlane(paged_visible(c, r0 / G));
     const uint32_t vis_max = __builtin_amdgcn_readfirstlane(paged_visible(c, r1 / G));
-
-    u32x4 qf[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      qf[s] = u32x4{0, 0, 0, 0};
-      if (live_row && qcol(s, g) < D)
-        qf[s] = ldg128(a.q + (c.first + qi) * a.q_stride + static_cast<uint64_t>(hq) * D +
-                       qcol(s, g));
-    }
-    f32x4 acc[NC];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) acc[i] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;   // m: the row's (all its lanes); l: this lane's positions
-    int ev = -1000;                  // f16 with codes: O is in units of 2^ev
-    char* const vlds = arena + wave * WB;
-
-    const uint32_t step = rows::UNIT;
     uint32_t base = k0 * rows::UNIT + wave * 32;
     const uint32_t end = min(static_cast<uint64_t>(k1) * rows::UNIT, static_cast<uint64_t>(vis_max));
-    Stage cur, nxt;
-    if (base < end) load(a, b, h, base, c.held, cur);
-    for (; base < end; base += step) {
-      if (base + step < end) load(a, b, h, base + step, c.held, nxt);
+    Stage st;
+    int32_t next[2];
+    if (base < end) {
+      pages(a, b, base, c.held, next);
+      load(a, h, base, end, next, st);
+      pages(a, b, base + rows::UNIT, c.held, next);
+    }
+
+    Sums y;
+    u32x4 qf[MT == 1 ? NS : 1];
+    uint32_t vis[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const uint32_t row = r0 + 16 * i + l16;
+      const bool live = row < nrows;
+      const uint32_t qi = live ? row / G : 0u, hq = h * G + (live ? row % G : 0u);
+      vis[i] = live ? paged_visible(c, qi) : 0u;
+      const uint16_t* const qp =
+          a.q + (c.first + qi) * a.q_stride + static_cast<uint64_t>(hq) * D;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        if (MT > 1 && (i * NS + s) % 4 != static_cast<int>(wave)) continue;
+        u32x4 x = {0, 0, 0, 0};
+        if (live && qcol(s, g) < D) x = ldg128(qp + qcol(s, g));
+        if constexpr (MT == 1) qf[s] = x;
+        else q_lds[(i * NS + s) * 64 + lane] = x;
+      }
+#pragma unroll
+      for (int x = 0; x < NC; ++x) y.acc[i][x] = f32x4{0, 0, 0, 0};
+      y.m[i] = -INFINITY;
+      y.l[i] = 0.0f;
+      y.ev[i] = -1000;
+    }
+    char* const vlds = arena + wave * WB;
+    if constexpr (MT > 1) __syncthreads();   // (Q of a pair of tiles leaves no registers for V)
+
+    for (; base < end; base += rows::UNIT) {
       // scores: lane (row l16, g) has positions base + 16 t + 4 g + i
-      f32x4 s[2];
+      f32x4 s[MT][2];
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
-        s[tt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int f = 0; f < NS; ++f) s[tt] = mfma16x16x32<DT>(kfrag(cur, tt, f), qf[f], s[tt]);
+        for (int i = 0; i < MT; ++i) s[i][tt] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[tt][i] *= kCodes ? cur.ks[tt][i] * a.scale_log2 : a.scale_log2;
-      }
-      const bool hides = base + 32 > vis_min || !cur.there[0] || !cur.there[1];   // uniform
-      bool hid[2][4];
+        for (int f = 0; f < NS; ++f) {
+          const u32x4 kf = kfrag(st, tt, f);
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          hid[tt][i] = hides && (base + 16 * tt + 4 * g + i >= vis || !cur.there[tt]);
-          if (hid[tt][i]) s[tt][i] = -INFINITY;
-        }
-      float mx = s[0][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[i >> 2][i & 3]);
-      float alpha = 1.0f;
-      bool moved = false;
-      if (__builtin_amdgcn_ballot_w64(mx > m + 8.0f) != 0) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
-        alpha = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
-        m = mn;
-        l *= alpha;
-        moved = true;
-      }
-      const float mu = m == -INFINITY ? 0.0f : m;
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = exp2_fast(s[i >> 2][i & 3] - mu);
-        l += p[i];
-      }
-      if constexpr (kCodes) {
-        float vs[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) vs[i] = hid[i >> 2][i & 3] ? 0.0f : cur.vs[i >> 2][i & 3];
-        if constexpr (DT == kF16) {
-          // f16 has five exponent bits: the scales enter relative to a power of two just above
-          // the largest that the row has seen
-          float big = vs[0];
-#pragma unroll
-          for (int i = 1; i < 8; ++i) big = fmaxf(big, vs[i]);
-          int e = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000;
-          if (__builtin_amdgcn_ballot_w64(e > ev) != 0) {
-            e = max(e, __shfl_xor(e, 16));
-            e = max(max(e, __shfl_xor(e, 32)), ev);
-            alpha *= __builtin_ldexpf(1.0f, max(ev - e, -300));
-            ev = e;
-            moved = true;
+          for (int i = 0; i < MT; ++i) {
+            const u32x4 x = MT == 1 ? qf[MT == 1 ? f : 0] : q_lds[(i * NS + f) * 64 + lane];
+            s[i][tt] = mfma16x16x32<DT>(kf, x, s[i][tt]);
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ev < -500 ? 0 : -ev);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] *= vs[i];
-      }
-      if (moved) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[i][j] *= alpha;
+          for (int x = 0; x < 4; ++x)
+            s[i][tt][x] *= kCodes ? st.ks[tt][x] * a.scale_log2 : a.scale_log2;
       }
-      const u32x4 pf = {pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
-                        pack2h<DT>(p[6], p[7])};
+      const bool there[2] = {st.page[0] >= 0, st.page[1] >= 0};
+      const bool hides = base + 32 > vis_min || !there[0] || !there[1];   // uniform
       bool odd = false;
       if (hides) {
 #pragma unroll
         for (int i = 0; i < VL; ++i)
-          odd |= base + i * (32 / VL) + lane / VROW < vis_max && any_nonfinite<CT>(cur.v[i]);
+          odd |= any_nonfinite<CT>(st.v[i]);
       }
-      if (__builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max) {
-        // NaN or infinities among values that some rows do not see (0 * NaN is NaN): these 32
-        // positions on the vector ALUs, each row over what it sees
-        lds_order();
-        put_v(cur, vlds, vis_max - base);
-        lds_order();
-#pragma unroll 1
-        for (int i = 0; i < 8; ++i) {
-#pragma unroll 1
-          for (int gk = 0; gk < 4; ++gk) {
-            const float pk = __shfl(p[0], l16 + 16 * gk);
-            const uint32_t r = 16 * (i >> 2) + 4 * gk + (i & 3);
-            if (base + r < vis) {
+      float vs[8];
+      if constexpr (kCodes) {
 #pragma unroll
-              for (int cc = 0; cc < NC; ++cc)
+        for (int i = 0; i < 8; ++i) vs[i] = st.vs[i >> 2][i & 3];
+      }
+      lds_order();
+      put_v(st, vlds);
+      lds_order();
+      if (base + rows::UNIT < end) {
+        load(a, h, base + rows::UNIT, end, next, st);
+        pages(a, b, base + 2 * rows::UNIT, c.held, next);
+      }
+
+      u32x4 pf[MT];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t d = 16 * cc + 4 * g + j;
-                  const uint16_t x = *reinterpret_cast<const uint16_t*>(
-                      vlds + vaddr(r, d >> 3) + 2 * (d & 7));
-                  acc[cc][j] = __builtin_fmaf(pk, u16_to_f32<DT>(x), acc[cc][j]);
-                }
+      for (int i = 0; i < MT; ++i) {
+        // of positions base + 16 (x / 4) + 4 g + x % 4, the row sees those below lim[x / 4]
+        int lim[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+          lim[tt] = there[tt] ? static_cast<int>(vis[i] - base) - 16 * tt - 4 * g : 0;
+        if (hides) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            s[i][x >> 2][x & 3] = (x & 3) < lim[x >> 2] ? s[i][x >> 2][x & 3] : -INFINITY;
+        }
+        float mx = s[i][0][0];
+#pragma unroll
+        for (int x = 1; x < 8; ++x) mx = fmaxf(mx, s[i][x >> 2][x & 3]);
+        float alpha = 1.0f;
+        bool moved = false;
+        if (__builtin_amdgcn_ballot_w64(mx > y.m[i] + 8.0f) != 0) {
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float mn = fmaxf(y.m[i], mx);
+          alpha = mn == -INFINITY ? 1.0f : exp2_fast(y.m[i] - mn);
+          y.m[i] = mn;
+          y.l[i] *= alpha;
+          moved = true;
+        }
+        const float mu = y.m[i] == -INFINITY ? 0.0f : y.m[i];
+        float p[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          p[x] = exp2_fast(s[i][x >> 2][x & 3] - mu);
+          y.l[i] += p[x];
+        }
+        if constexpr (kCodes) {
+          float w[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) w[x] = vs[x];
+          if (hides) {   // (a hidden token's scale may be NaN)
+#pragma unroll
+            for (int x = 0; x < 8; ++x) w[x] = (x & 3) < lim[x >> 2] ? vs[x] : 0.0f;
+          }
+          if constexpr (kExps) {
+            // f16 has five exponent bits: the scales enter relative to a power of two just above
+            // the largest that the row has seen
+            float big = w[0];
+#pragma unroll
+            for (int x = 1; x < 8; ++x) big = fmaxf(big, w[x]);
+            int e = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000;
+            if (__builtin_amdgcn_ballot_w64(e > y.ev[i]) != 0) {
+              e = max(e, __shfl_xor(e, 16));
+              e = max(max(e, __shfl_xor(e, 32)), y.ev[i]);
+              alpha *= __builtin_ldexpf(1.0f, max(y.ev[i] - e, -300));
+              y.ev[i] = e;
+              moved = true;
             }
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              w[x] = __builtin_ldexpf(w[x], y.ev[i] < -500 ? 0 : -y.ev[i]);
           }
 #pragma unroll
-          for (int j = 0; j < 7; ++j) p[j] = p[j + 1];
+          for (int x = 0; x < 8; ++x) p[x] *= w[x];
         }
-      } else {
-        lds_order();
-        put_v(cur, vlds, vis_max - base);
-        lds_order();
-        pv(vlds, pf, acc);
+        if (moved) {
+#pragma unroll
+          for (int x = 0; x < NC; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y.acc[i][x][j] *= alpha;
+        }
+        pf[i] = u32x4{pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
+                      pack2h<DT>(p[6], p[7])};
       }
-      cur = nxt;
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if constexpr (kCodes && DT == kF16) {
+      if (__builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max) {
+        // NaN or infinities among values that some rows do not see (0 * NaN is NaN)
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = ev < -500 ? 0.0f : __builtin_ldexpf(acc[i][j], ev);
+        for (int i = 0; i < MT; ++i)
+          pv_seen(vlds, pf[i], vis[i] > base ? vis[i] - base : 0u, y.acc[i]);
+      } else {
+        pv(vlds, pf, y);
+      }
     }
 
     // the four waves' sums
-    __shared__ float sm[4][rows::TR], sl[4][rows::TR];
+    __shared__ float sm[4][TR], sl[4][TR];
     lds_order();
     float* wo = reinterpret_cast<float*>(vlds);
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      *reinterpret_cast<f32x4*>(wo + l16 * ORS + 16 * i + 4 * g) = acc[i];
-    if (g == 0) {
-      sm[wave][l16] = m;
-      sl[wave][l16] = l;
+    for (int i = 0; i < MT; ++i) {
+      float l = y.l[i];
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+#pragma unroll
+      for (int x = 0; x < NC; ++x) {
+        if constexpr (kExps) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y.acc[i][x][j] = y.ev[i] < -500 ? 0.0f : __builtin_ldexpf(y.acc[i][x][j], y.ev[i]);
+        }
+        *reinterpret_cast<f32x4*>(wo + (16 * i + l16) * ORS + 16 * x + 4 * g) = y.acc[i][x];
+      }
+      if (g == 0) {
+        sm[wave][16 * i + l16] = y.m[i];
+        sl[wave][16 * i + l16] = l;
+      }
     }
     __syncthreads();
     constexpr int CPR = HD / 8;   // 8-value pieces of a row
-    for (int x = t; x < rows::TR * CPR; x += rows::NT) {
+    for (int x = t; x < TR * CPR; x += rows::NT) {
       const int r = x / CPR, c8 = 8 * (x % CPR);
       if (r0 + r >= nrows || c8 >= static_cast<int>(D)) continue;
-      float M = sm[0][r], w[4], ls = 0.0f, o[8];
+      float M = sm[0][r], ls = 0.0f, o[8];
 #pragma unroll
       for (int i = 1; i < 4; ++i) M = fmaxf(M, sm[i][r]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = sm[i][r] == -INFINITY ? 0.0f : exp2_fast(sm[i][r] - M);
-        ls = sl[i][r] != 0.0f ? __builtin_fmaf(w[i], sl[i][r], ls) : ls;
-      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[j] = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float* src = reinterpret_cast<const float*>(arena + i * WB) + r * ORS + c8;
         if (sl[i][r] == 0.0f) continue;   // a wave that saw nothing
+        const float w = sm[i][r] == -INFINITY ? 0.0f : exp2_fast(sm[i][r] - M);
+        const float* src = reinterpret_cast<const float*>(arena + i * WB) + r * ORS + c8;
+        ls = __builtin_fmaf(w, sl[i][r], ls);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = __builtin_fmaf(w[i], src[j], o[j]);
+        for (int j = 0; j < 8; ++j) o[j] = __builtin_fmaf(w, src[j], o[j]);
       }
       if (part) {
         *reinterpret_cast<f32x4*>(part + r * HD + c8) = f32x4{o[0], o[1], o[2], o[3]};
         *reinterpret_cast<f32x4*>(part + r * HD + c8 + 4) = f32x4{o[4], o[5], o[6], o[7]};
         if (c8 == 0) {
-          part[rows::TR * HD + r] = M;
-          part[rows::TR * HD + rows::TR + r] = ls;
+          part[TR * HD + r] = M;
+          part[TR * HD + TR + r] = ls;
         }
       } else {
-        write_row(a, c, h, r0 + r, c8, o, ls);
+        write_row<DT>(a, c, h, r0 + r, c8, o, ls);
       }
     }
     __syncthreads();   // the arena and the statistics serve the run's next tile
   }
-
-  static __device__ __forceinline__ void write_row(const AttnArgs& a, const PagedChunk& c,
-                                                   uint32_t h, uint32_t row, int c8,
-                                                   const float (&o)[8], float l) {
-    const uint64_t tok = c.first + row / a.group;
-    const uint32_t hq = h * a.group + row % a.group;
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = l == 0.0f ? 0.0f : o[j] / l;
-    *reinterpret_cast<u32x4*>(a.o + (tok * a.nh + hq) * a.pool.head_dim + c8) =
-        u32x4{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3]), pack2h<DT>(f[4], f[5]),
-              pack2h<DT>(f[6], f[7])};
-  }
 };
 
-template <int DT, int CT, int HD>
-__global__ void __launch_bounds__(rows::NT, 2)
+// Waves per SIMD that the registers of a tile's kernel are kept to.
+template <int HD, int MT> constexpr int rows_waves() { return HD == 256 ? 1 : 2; }
+
+template <int DT, int CT, int HD, int MT>
+__global__ void __launch_bounds__(rows::NT, (rows_waves<HD, MT>()))
 attn_paged_rows(AttnArgs a) {
-  using T = RowsTile<DT, CT, HD>;
+  using T = RowsTile<DT, CT, HD, MT>;
   __shared__ __align__(16) char arena[4 * T::WB];
-  const uint64_t units = scan_units(a, [](uint32_t, uint64_t, uint64_t, uint64_t) {});
+  __shared__ u32x4 q_lds[MT > 1 ? MT * T::NS * 64 : 1];
+  Place at(a);
   const uint32_t w = blockIdx.x, nw = gridDim.x;
-  const uint64_t u1 = run_start(units, w + 1, nw);
-  uint64_t u = run_start(units, w, nw);
-  if (u >= u1) return;
-  Where at = find_unit(a, u);
-  while (u < u1 && at.b < a.seqs.batch) {
-    const PagedChunk c = paged_chunk(a.seqs, at.b);
-    const SeqWork sw = rows_work(a, c);
-    const uint64_t all = static_cast<uint64_t>(sw.tiles) * sw.units * a.pool.nkv;
-    if (all == 0) {
-      ++at.b;
-      continue;
-    }
-    while (u < u1 && u < at.before + all) {
-      const uint64_t in = u - at.before;
-      const uint32_t k0 = static_cast<uint32_t>(in % sw.units);
-      const uint64_t th_ = in / sw.units;
-      const uint32_t h = static_cast<uint32_t>(th_ % a.pool.nkv);
-      const uint32_t tile = static_cast<uint32_t>(th_ / a.pool.nkv);
-      const uint32_t k1 =
-          static_cast<uint32_t>(min(static_cast<uint64_t>(sw.units), k0 + (u1 - u)));
+  const uint64_t u1 = run_start(at.units, w + 1, nw);
+  uint64_t u = run_start(at.units, w, nw);
+  while (u < u1) {
+    if (!at.find(a, u)) return;
+    const PagedChunk c = at.chunk();
+    const uint32_t blocks = read_lane(at.g.blocks, at.l);
+    const uint64_t upto = read_lane64(at.g.upto, at.l);
+    const uint64_t before = upto - read_lane64(at.g.units, at.l);
+    while (u < u1 && u < upto) {
+      const uint64_t in = u - before;
+      // (divisions leave what all lanes share in vector registers: back to scalar ones)
+      const uint64_t item = in / blocks;
+      const uint32_t k0 =
+          __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(in - item * blocks));
+      const uint32_t h = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(item % a.pool.nkv));
+      const uint32_t tile =
+          __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(item / a.pool.nkv));
+      const uint32_t k1 = __builtin_amdgcn_readfirstlane(
+          static_cast<uint32_t>(min(static_cast<uint64_t>(blocks), k0 + (u1 - u))));
       float* part = nullptr;
-      if (k0 != 0 || k1 != sw.units)
-        part = a.ws + (2ull * w + (k0 == 0 ? 1 : 0)) * rows::rec(HD);
-      T::run(a, c, at.b, h, tile, k0, k1, part, arena);
+      if (k0 != 0 || k1 != blocks)
+        part = a.ws + (2ull * w + (k0 == 0 ? 1 : 0)) * rows::rec(HD, T::TR);
+      T::run(a, c, at.b0 + at.l, h, tile, k0, k1, part, arena, q_lds);
       u += k1 - k0;
     }
-    at.before += all;
-    ++at.b;
   }
 }
 
-// Merge the parts of tiles that several runs share.  Workgroup w looks after the tile in which
+// Merge the parts of a tile that several runs share.  Workgroup w looks after the tile in which
 // run w + 1 begins, if run w holds that tile's first unit: parts 2 w + 1, then 2 (w + 1), ...
-// One wave per row.
-template <int DT, int CT, int HD>
-__global__ void __launch_bounds__(256)
-attn_paged_merge(AttnArgs a, uint32_t nw) {
-  using T = RowsTile<DT, CT, HD>;
-  const uint64_t units = scan_units(a, [](uint32_t, uint64_t, uint64_t, uint64_t) {});
-  const uint32_t w = blockIdx.x;
-  const uint64_t u = run_start(units, w + 1, nw);
-  if (u >= units) return;
-  const Where at = find_unit(a, u);
-  if (at.b >= a.seqs.batch) return;
-  const PagedChunk c = paged_chunk(a.seqs, at.b);
-  const SeqWork sw = rows_work(a, c);
-  const uint64_t in = u - at.before;
-  const uint64_t item0 = u - in % sw.units, item1 = item0 + sw.units;
-  if (item0 == u || run_start(units, w, nw) > item0) return;
-  uint32_t last = w + 1;   // the last run with a unit of the tile
-  while (last + 1 < nw && run_start(units, last + 1, nw) < item1) ++last;
-  const uint64_t th_ = in / sw.units;
-  const uint32_t h = static_cast<uint32_t>(th_ % a.pool.nkv);
-  const uint32_t r0 = static_cast<uint32_t>(th_ / a.pool.nkv) * rows::TR, nrows = c.n * a.group;
+// One wave per row, HD / 8 lanes per part of it.
+template <int DT, int HD>
+__device__ __forceinline__ void rows_merge(const AttnArgs& a, uint32_t w) {
+  Place at(a);
+  const uint32_t nw = a.runs, TR = a.tile_rows;
+  const uint64_t u = run_start(at.units, w + 1, nw);
+  if (u >= at.units || !at.find(a, u)) return;
+  const PagedChunk c = at.chunk();
+  const uint32_t blocks = read_lane(at.g.blocks, at.l);
+  const uint64_t before = read_lane64(at.g.upto, at.l) - read_lane64(at.g.units, at.l);
+  const uint64_t item = (u - before) / blocks;
+  const uint64_t item0 = before + item * blocks, item1 = item0 + blocks;
+  if (item0 == u || run_start(at.units, w, nw) > item0) return;
+  // the last run with a unit of the tile
+  const uint64_t each = at.units / nw, more = at.units % nw, lastu = item1 - 1;
+  const uint32_t last = static_cast<uint32_t>(
+      lastu < (each + 1) * more ? lastu / (each + 1) : more + (lastu - (each + 1) * more) / each);
+  const uint32_t h = static_cast<uint32_t>(item % a.pool.nkv);
+  const uint32_t r0 = static_cast<uint32_t>(item / a.pool.nkv) * TR, nrows = c.n * a.group;
   const uint32_t np = last - w + 1;
-  auto rec = [&](uint32_t i) {
-    return a.ws + (i == 0 ? 2ull * w + 1 : 2ull * (w + i)) * rows::rec(HD);
-  };
+  const int size = rows::rec(HD, static_cast<int>(TR));
+  auto rec = [&](uint32_t i) { return a.ws + (i == 0 ? 2ull * w + 1 : 2ull * (w + i)) * size; };
   const int lane = threadIdx.x & 63;
   constexpr int CPR = HD / 8, PG = 64 / CPR;   // parts that a wave reads at once
   const int c8 = 8 * (lane % CPR), pg = lane / CPR;
-  for (int r = threadIdx.x >> 6; r < rows::TR && r0 + r < nrows; r += 4) {
-    float M = -INFINITY;
-    for (uint32_t i = lane; i < np; i += 64) M = fmaxf(M, rec(i)[rows::TR * HD + r]);
-    M = wave_max(M);
-    float o[8], ls = 0.0f;
+  for (uint32_t r = threadIdx.x >> 6; r < TR && r0 + r < nrows; r += 4) {
+    float M = -INFINITY, o[8], ls = 0.0f;
+    for (uint32_t i = lane; i < np; i += 64) M = fmaxf(M, rec(i)[TR * HD + r]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[j] = 0.0f;
+    M = wave_max(M);
+#pragma unroll 4
     for (uint32_t i = pg; i < np; i += PG) {
       const float* p = rec(i);
-      const float m = p[rows::TR * HD + r], l = p[rows::TR * HD + rows::TR + r];
-      if (l == 0.0f) continue;
-      const float wt = m == -INFINITY ? 0.0f : exp2_fast(m - M);
-      ls = __builtin_fmaf(wt, l, ls);
+      const float m = p[TR * HD + r], l = p[TR * HD + TR + r];
       const f32x4 x = *reinterpret_cast<const f32x4*>(p + r * HD + c8);
       const f32x4 y = *reinterpret_cast<const f32x4*>(p + r * HD + c8 + 4);
+      const float wt = m == -INFINITY ? 0.0f : exp2_fast(m - M);
+      if (l != 0.0f) {   // (else the part saw nothing)
+        ls = __builtin_fmaf(wt, l, ls);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        o[j] = __builtin_fmaf(wt, x[j], o[j]);
-        o[4 + j] = __builtin_fmaf(wt, y[j], o[4 + j]);
+        for (int j = 0; j < 4; ++j) {
+          o[j] = __builtin_fmaf(wt, x[j], o[j]);
+          o[4 + j] = __builtin_fmaf(wt, y[j], o[4 + j]);
+        }
       }
     }
 #pragma unroll
@@ -632,7 +733,7 @@ attn_paged_merge(AttnArgs a, uint32_t nw) {
       for (int j = 0; j < 8; ++j) o[j] += __shfl_xor(o[j], d);
     }
     if (pg == 0 && c8 < static_cast<int>(a.pool.head_dim))
-      T::write_row(a, c, h, r0 + r, c8, o, ls);
+      write_row<DT>(a, c, h, r0 + r, c8, o, ls);
   }
 }
 
@@ -735,8 +836,8 @@ attn_paged_chunk(AttnArgs a) {
 
   // item: heads fastest (workgroup w runs on XCD w % 8, so a head's tiles share an L2 where
   // there are eight), then parts, then tiles from the last (longest) on, then sequences
-  const uint32_t h = blockIdx.x % nkv;
-  const uint32_t part = blockIdx.x / nkv % a.parts;
+  const uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.x % nkv);
+  const uint32_t part = __builtin_amdgcn_readfirstlane(blockIdx.x / nkv % a.parts);
   uint32_t left = blockIdx.x / nkv / a.parts, b = 0;
   {
     bool found = false;
@@ -766,7 +867,7 @@ attn_paged_chunk(AttnArgs a) {
   const PagedChunk c = paged_chunk(a.seqs, b);
   const uint32_t nrows = c.n * G;
   const uint32_t reach = __builtin_amdgcn_readfirstlane(tile_reach(a, c, tile));
-  const uint32_t per = part_blocks(reach, a.parts);
+  const uint32_t per = __builtin_amdgcn_readfirstlane(part_blocks(reach, a.parts));
   const uint32_t nb_all = (reach + KB - 1) / KB;
   const uint32_t j0 = part * per, j1 = min(nb_all, j0 + per);
   if (part != 0 && j0 >= nb_all) return;
@@ -803,47 +904,47 @@ attn_paged_chunk(AttnArgs a) {
   int ev = -1000;   // f16 with codes: O is in units of 2^ev
   if (t < 2) sh.odd[t] = 0xffffffffu;
 
-  // this thread's pieces of a block: rows xr, 16-byte pieces xc
-  uint32_t xr[XPT], xc[XPT];
+  // this thread's pieces of a block: rows xr, 16-byte pieces xc.  A wave's rows, from wr on, lie
+  // in one group of 16, so in one page.
+  static_assert(64 / T::CPR <= 16, "a wave's rows lie in one page");
+  uint32_t xr[XPT], xc[XPT], wr[XPT];
 #pragma unroll
   for (int i = 0; i < XPT; ++i) {
     const uint32_t x = min(static_cast<uint32_t>(t + NT * i), static_cast<uint32_t>(T::NX - 1));
     xr[i] = x / T::CPR;
     xc[i] = x % T::CPR;
+    wr[i] = __builtin_amdgcn_readfirstlane(xr[i]) & ~(64u / T::CPR - 1);
   }
   const uint32_t rb = D * T::ESZ;
   typename T::Stage st;
   int32_t id[XPT], id_s = -1;       // pages of the next block to be loaded
-  uint32_t ok = 0, ok_next = 0;     // which of the stage's pieces are held (bit XPT: the scale)
+  bool ok[XPT];                     // the stage's pages exist
   auto pages = [&](uint32_t j) {
     const uint32_t base = j * KB;
 #pragma unroll
     for (int i = 0; i < XPT; ++i)
-      id[i] = base + xr[i] < reach ? paged_page(a.seqs, b, base + xr[i]) : -1;
+      id[i] = base + wr[i] < reach ? wave_page(a.seqs, b, base + wr[i]) : -1;
     if constexpr (T::kCodes)
       id_s = t < 2 * KB && base + (t & 63) < reach ? paged_page(a.seqs, b, base + (t & 63)) : -1;
   };
+  // Rows of missing pages and from `reach` on come as zeros, scales too.
   auto load = [&](uint32_t j) {
     const uint32_t base = j * KB;
-    const char* kp = static_cast<const char*>(a.pool.k);
-    const char* vp = static_cast<const char*>(a.pool.v);
-    ok_next = 0;
 #pragma unroll
     for (int i = 0; i < XPT; ++i) {
-      ok_next |= id[i] >= 0 ? 1u << i : 0u;
-      const uint64_t at =
-          pool_row(a.pool, a.seqs, max(id[i], 0), h,
-                   id[i] >= 0 ? paged_row(a.seqs, base + xr[i]) : 0u) * T::ESZ +
-          min(16u * xc[i], rb - 16);
-      st.k[i] = ldg128(kp + at);
-      st.v[i] = ldg128(vp + at);
+      const uint32_t pos = base + wr[i];
+      const uint32_t n = id[i] >= 0 && pos < reach ? min(64u / T::CPR, reach - pos) : 0u;
+      const uint64_t at = pool_row(a.pool, a.seqs, max(id[i], 0), h, paged_row(a.seqs, pos)) * T::ESZ;
+      const uint32_t off = 16 * xc[i] < rb ? (xr[i] - wr[i]) * rb + 16 * xc[i] : kPast;
+      st.k[i] = load_within<false>(static_cast<const char*>(a.pool.k) + at, n * rb, off);
+      st.v[i] = load_within<false>(static_cast<const char*>(a.pool.v) + at, n * rb, off);
+      ok[i] = id[i] >= 0;
     }
     if constexpr (T::kCodes) {
-      if (id_s >= 0) {
-        ok_next |= 1u << XPT;
+      st.scale = 0.0f;
+      if (id_s >= 0)
         st.scale = (t < KB ? a.pool.k_scale : a.pool.v_scale)[pool_scale(
             a.pool, a.seqs, id_s, h, paged_row(a.seqs, base + (t & 63)))];
-      }
     }
   };
   auto store = [&](uint32_t j) {   // what load(j) brought
@@ -853,34 +954,25 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < XPT; ++i) {
       if (T::NX < NT && t >= T::NX) break;
-      u32x4 k = st.k[i], v = st.v[i];
+      const u32x4 k = st.k[i], v = st.v[i];
       const uint32_t r = xr[i], cc = xc[i];
-      if (16 * cc >= rb) k = u32x4{0, 0, 0, 0};   // (Q is zero there, K may be infinite)
-      if (!(ok >> i & 1)) v = u32x4{0, 0, 0, 0};
       odd |= any_nonfinite<CT>(v);
       if constexpr (T::kCodes) {
-        u32x2 w[8];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          w[x] = widen4<DT, CT>(k[x]);
-          w[4 + x] = widen4<DT, CT>(v[x]);
-        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          *reinterpret_cast<u32x4*>(kl + T::kaddr(r, 2 * cc + x)) =
-              u32x4{w[2 * x][0], w[2 * x][1], w[2 * x + 1][0], w[2 * x + 1][1]};
-          *reinterpret_cast<u32x4*>(vl + T::vaddr(r, 2 * cc + x)) =
-              u32x4{w[4 + 2 * x][0], w[4 + 2 * x][1], w[5 + 2 * x][0], w[5 + 2 * x][1]};
+          const u32x2 k0 = widen4<DT, CT>(k[2 * x]), k1 = widen4<DT, CT>(k[2 * x + 1]);
+          *reinterpret_cast<u32x4*>(kl + T::kaddr(r, 2 * cc + x)) = u32x4{k0[0], k0[1], k1[0], k1[1]};
+          const u32x2 v0 = widen4<DT, CT>(v[2 * x]), v1 = widen4<DT, CT>(v[2 * x + 1]);
+          *reinterpret_cast<u32x4*>(vl + T::vaddr(r, 2 * cc + x)) = u32x4{v0[0], v0[1], v1[0], v1[1]};
         }
       } else {
         *reinterpret_cast<u32x4*>(kl + T::kaddr(r, cc)) = k;
         *reinterpret_cast<u32x4*>(vl + T::vaddr(r, cc)) = v;
       }
-      if (cc == 0 && (r & 15) == 0) sh.there[j & 1][r >> 4] = ok >> i & 1;
+      if (cc == 0 && (r & 15) == 0) sh.there[j & 1][r >> 4] = ok[i];
     }
     if constexpr (T::kCodes) {
-      if (t < 2 * KB)
-        (t < KB ? sh.ks : sh.vs)[j & 1][t & 63] = ok >> XPT & 1 ? st.scale : 0.0f;
+      if (t < 2 * KB) (t < KB ? sh.ks : sh.vs)[j & 1][t & 63] = st.scale;
     }
     if (odd && (j + 1) * KB > tile_min) sh.odd[j & 1] = j;   // (any of them: one value)
   };
@@ -931,7 +1023,8 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
-          if (at >= lim || !(there >> (at >> 4) & 1)) s[kt][i] = -INFINITY;
+          const int lim_g = there >> (at >> 4) & 1 ? lim : -64;   // (uniform)
+          s[kt][i] = at < lim_g ? s[kt][i] : -INFINITY;
         }
     }
     float mx[4];
@@ -984,24 +1077,6 @@ attn_paged_chunk(AttnArgs a) {
           moved = true;
         }
       }
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][32 * kt + 8 * q + 4 * g]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == kF16) vs[i] = __builtin_ldexpf(vs[i], ev < -500 ? 0 : -ev);
-            s[kt][4 * q + i] *= vs[i];
-          }
-        }
-      if (hides) {   // (a hidden token's scale may be NaN)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * kt + 8 * (i >> 2) + (i & 3) >= lim) s[kt][i] = 0.0f;
-      }
     }
     if (moved) {
 #pragma unroll
@@ -1009,7 +1084,26 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
         for (int x = 0; x < 16; ++x) acc[i][x] *= alpha;
     }
+    // the probabilities of PV step sp, by their positions' scales
+    auto weigh = [&](int sp) {
+      if constexpr (T::kCodes) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int at = 16 * sp + 8 * q;
+          f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][at + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (DT == kF16) vs[i] = __builtin_ldexpf(vs[i], ev < -500 ? 0 : -ev);
+            const int x = 8 * (sp & 1) + 4 * q + i;
+            s[sp >> 1][x] *= vs[i];
+            if (hides) s[sp >> 1][x] = at + i < lim ? s[sp >> 1][x] : 0.0f;   // (may be NaN)
+          }
+        }
+      }
+    };
     if (hides && __builtin_amdgcn_readfirstlane(sh.odd[j & 1]) == j && vis_min < reach) {
+#pragma unroll
+      for (int sp = 0; sp < 4; ++sp) weigh(sp);
       // NaN or infinities among values that some rows do not see (0 * NaN is NaN): this block on
       // the vector ALUs, each row over what it sees
 #pragma unroll 1
@@ -1020,14 +1114,18 @@ attn_paged_chunk(AttnArgs a) {
           const uint32_t r = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * gk + (i & 3);
           if (base + r < vis) {
 #pragma unroll
-            for (int dt = 0; dt < T::NDT; ++dt)
+            for (int x = 0; x < 4 * T::NDT; ++x) {
+              uint32_t dg = 4 * g;
+              asm volatile("" : "+v"(dg) : : "memory");   // (few registers, as for the rows)
+              const uint32_t d = 8 * x + dg;
+              const u32x2 v =
+                  *reinterpret_cast<const u32x2*>(vl + T::vaddr(r, d >> 3) + 2 * (d & 7));
 #pragma unroll
-              for (int x = 0; x < 16; ++x) {
-                const uint32_t d = 32 * dt + 8 * (x >> 2) + 4 * g + (x & 3);
-                const uint16_t v =
-                    *reinterpret_cast<const uint16_t*>(vl + T::vaddr(r, d >> 3) + 2 * (d & 7));
-                acc[dt][x] = __builtin_fmaf(pk, u16_to_f32<DT>(v), acc[dt][x]);
-              }
+              for (int y = 0; y < 4; ++y)
+                acc[x >> 2][4 * (x & 3) + y] = __builtin_fmaf(
+                    pk, u16_to_f32<DT>(static_cast<uint16_t>(v[y >> 1] >> (16 * (y & 1)))),
+                    acc[x >> 2][4 * (x & 3) + y]);
+            }
           }
         }
 #pragma unroll
@@ -1038,6 +1136,7 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
     for (int sp = 0; sp < 4; ++sp) {
       const int o = 8 * (sp & 1);
+      weigh(sp);
       const f32x16& p = s[sp >> 1];
       const u32x4 pf = {pack2h<DT>(p[o], p[o + 1]), pack2h<DT>(p[o + 2], p[o + 3]),
                         pack2h<DT>(p[o + 4], p[o + 5]), pack2h<DT>(p[o + 6], p[o + 7])};
@@ -1055,14 +1154,12 @@ attn_paged_chunk(AttnArgs a) {
   if (j0 < j1) {
     pages(j0);
     load(j0);
-    ok = ok_next;
     if (j0 + 1 < j1) pages(j0 + 1);
     __syncthreads();   // (sh.odd)
     store(j0);
     if (j0 + 1 < j1) {
       load(j0 + 1);
-      ok = ok_next;
-    }
+      }
     if (j0 + 2 < j1) pages(j0 + 2);
     for (uint32_t j = j0; j < j1; ++j) {
       // block j is whole in LDS, and every wave is done with block j - 1, whose half block
@@ -1071,8 +1168,7 @@ attn_paged_chunk(AttnArgs a) {
       if (j + 1 < j1) store(j + 1);
       if (j + 2 < j1) {
         load(j + 2);
-        ok = ok_next;
-      }
+          }
       if (j + 3 < j1) pages(j + 3);
       compute(j);
     }
@@ -1121,11 +1217,10 @@ attn_paged_chunk(AttnArgs a) {
 
 // Merge a chunk tile's parts: one workgroup per token, HD / 4 lanes per row.
 template <int DT, int HD>
-__global__ void __launch_bounds__(256)
-attn_paged_chunk_merge(AttnArgs a) {
+__device__ __forceinline__ void chunk_merge(const AttnArgs& a, uint32_t token) {
   using namespace chunk;
   constexpr int LPR = HD / 4, RPB = 256 / LPR;
-  const uint32_t lane = threadIdx.x & 63u, token = blockIdx.x;
+  const uint32_t lane = threadIdx.x & 63u;
   uint32_t le = 0;
   for (uint32_t j0 = 0; j0 < a.seqs.batch; j0 += 64) {
     const uint32_t j = j0 + lane;
@@ -1163,6 +1258,17 @@ attn_paged_chunk_merge(AttnArgs a) {
       *reinterpret_cast<u32x2*>(a.o + (static_cast<uint64_t>(token) * a.nh + hq) * a.pool.head_dim +
                                 d) = u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
     }
+  }
+}
+
+// Both kernels' merges in one launch: `first` workgroups for the rows' runs, then one per token.
+template <int DT, int HD>
+__global__ void __launch_bounds__(256)
+attn_paged_merge(AttnArgs a, uint32_t first) {
+  if (blockIdx.x < first) {
+    rows_merge<DT, HD>(a, blockIdx.x);
+  } else if constexpr (HD <= 128) {
+    chunk_merge<DT, HD>(a, blockIdx.x - first);
   }
 }
 

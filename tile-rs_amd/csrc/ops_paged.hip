@@ -105,15 +105,17 @@ uint32_t head_width(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <
 // How a call is split over its kernels, from what the host knows: the structs' sizes.
 struct AttnPlan {
   uint32_t runs = 0;         // workgroups of the rows' kernel (0: not launched)
+  uint32_t tile_rows = 16;
+  bool rows_merge = false;
   uint32_t split_rows = 0;   // sequences of more rows go to the chunks' kernel
   uint64_t items = 0;        // (tile, head) items of the chunks' kernel, at most (0: not launched)
   uint32_t parts = 1;
   size_t rows_bytes = 0, chunk_bytes = 0;
 };
 
-// Runs that the rows' units are dealt to: two workgroups per CU.  CUs of a whole MI355X, not of
-// the current device, so that the workspace's size does not depend on it.
-constexpr uint32_t kCus = 256, kMaxRuns = 2 * kCus;
+// CUs of a whole MI355X, not of the current device, so that the workspace's size does not
+// depend on it.
+constexpr uint32_t kCus = 256;
 // Rows up to which a sequence stays with the rows' kernel.
 constexpr uint32_t kSplitRows = 64;
 
@@ -125,14 +127,19 @@ AttnPlan attn_plan(const th::PagedSeqs& s, uint32_t nkv, uint32_t group, uint32_
   const bool chunks = hd <= 128 && rows > kSplitRows && s.total_q > s.batch;
   p.split_rows = !chunks ? 0xffffffffu : s.batch == 1 ? 0u : kSplitRows;
   if (p.split_rows != 0) {
+    if (hd <= 128 && rows > 16ull * s.batch) p.tile_rows = 32;
     // at least the units of any lengths that the structs allow
-    const uint64_t tiles = rows / th::pgd::rows::TR + s.batch;
+    const uint64_t tiles = rows / p.tile_rows + s.batch;
     const uint64_t cap = uint64_t{1} << 40;
-    const uint64_t units =
-        std::min(cap, std::min(cap, tiles * nkv) * (s.cap / th::pgd::rows::UNIT + 1));
-    p.runs = static_cast<uint32_t>(std::min<uint64_t>(kMaxRuns, units));
-    p.rows_bytes =
-        static_cast<size_t>(p.runs) * 2 * th::pgd::rows::rec(static_cast<int>(hd)) * sizeof(float);
+    const uint64_t blocks = s.cap / th::pgd::rows::UNIT + (s.cap % th::pgd::rows::UNIT != 0);
+    const uint64_t units = std::min(cap, std::min(cap, tiles * nkv) * std::max<uint64_t>(1, blocks));
+    const uint32_t per_cu = hd == 256 ? 1 : 2;   // (rows_waves)
+    p.runs = static_cast<uint32_t>(std::min<uint64_t>(per_cu * kCus, units));
+    p.rows_merge = p.runs > 1 && blocks > 1;
+    if (p.rows_merge)
+      p.rows_bytes = static_cast<size_t>(p.runs) * 2 *
+                     th::pgd::rows::rec(static_cast<int>(hd), static_cast<int>(p.tile_rows)) *
+                     sizeof(float);
   }
   if (chunks) {
     const uint64_t some = rows / (p.split_rows + 1);   // sequences of more than split_rows rows
@@ -151,23 +158,23 @@ AttnPlan attn_plan(const th::PagedSeqs& s, uint32_t nkv, uint32_t group, uint32_
 
 template <int DT, int CT, int HD>
 void attn_paged_go(const th::pgd::AttnArgs& a, const AttnPlan& p, hipStream_t s) {
-  if (p.runs) {
-    hipLaunchKernelGGL((th::pgd::attn_paged_rows<DT, CT, HD>), dim3(p.runs),
-                       dim3(th::pgd::rows::NT), 0, s, a);
-    if (p.runs > 1)
-      hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, CT, HD>), dim3(p.runs - 1), dim3(256), 0,
-                         s, a, p.runs);
-  }
+  constexpr uint32_t NT = th::pgd::rows::NT;
+  if (p.runs && p.tile_rows == 16)
+    hipLaunchKernelGGL((th::pgd::attn_paged_rows<DT, CT, HD, 1>), dim3(p.runs), dim3(NT), 0, s, a);
   if constexpr (HD <= 128) {
-    if (p.items) {
+    if (p.runs && p.tile_rows == 32)
+      hipLaunchKernelGGL((th::pgd::attn_paged_rows<DT, CT, HD, 2>), dim3(p.runs), dim3(NT), 0, s,
+                         a);
+    if (p.items)
       hipLaunchKernelGGL((th::pgd::attn_paged_chunk<DT, CT, HD>),
                          dim3(static_cast<uint32_t>(p.items * p.parts)), dim3(th::pgd::chunk::NT),
                          0, s, a);
-      if (p.parts > 1)
-        hipLaunchKernelGGL((th::pgd::attn_paged_chunk_merge<DT, HD>), dim3(a.seqs.total_q),
-                           dim3(256), 0, s, a);
-    }
   }
+  const uint32_t first = p.rows_merge ? p.runs - 1 : 0;
+  const uint32_t tokens = p.items && p.parts > 1 ? a.seqs.total_q : 0;
+  if (first + tokens)   // below 2^31: total_q and a few runs
+    hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, HD>), dim3(first + tokens), dim3(256), 0, s,
+                       a, first);
 }
 
 }  // namespace
@@ -294,7 +301,9 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
   }
   a.ws = static_cast<float*>(workspace);
   a.chunk_ws = a.ws + plan.rows_bytes / sizeof(float);
+  a.tile_rows = plan.tile_rows;
   a.split_rows = plan.split_rows;
+  a.runs = plan.runs;
   a.parts = plan.parts;
   auto go = [&](auto dt, auto ct) {
     switch (head_width(D)) {
