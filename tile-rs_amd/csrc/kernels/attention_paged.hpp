@@ -86,6 +86,15 @@ __device__ __forceinline__ u32x4 load_within(const void* p, uint32_t bytes, uint
 // An offset that is past every range.
 constexpr uint32_t kPast = 0x7ffffff0u;
 
+// f16 probabilities times scales need not fit f16's five exponent bits.  So the scores of a row
+// are taken relative to its maximum plus the exponent of the largest scale that it has seen (at
+// least kLeastExp, so that f32 holds the rest): products are then at most 2^8 as without scales,
+// and numerator and denominator share the factor.
+constexpr float kLeastExp = -100.0f;
+__device__ __forceinline__ float scale_exp(float most) {
+  return most > 0.0f ? static_cast<float>(__builtin_amdgcn_frexp_expf(most)) : kLeastExp;
+}
+
 // Whether a NaN or an infinity is among the 16 bytes.
 template <int CT>
 __device__ __forceinline__ bool any_nonfinite(u32x4 v) {
@@ -244,7 +253,7 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, const PagedChunk& c
 template <int DT, int CT, int HD, int MT>
 struct RowsTile {
   static constexpr bool kCodes = cache_codes<CT>();
-  static constexpr bool kExps = kCodes && DT == kF16;   // scales enter relative to 2^ev
+  static constexpr bool kExps = kCodes && DT == kF16;   // (scale_exp)
   static constexpr int ESZ = cache_size<CT>();
   static constexpr int TR = 16 * MT;
   static constexpr int NS = HD / 32;             // K fragments (32 values deep) of a position
@@ -266,8 +275,8 @@ struct RowsTile {
   };
   struct Sums {
     f32x4 acc[MT][NC];
-    float m[MT], l[MT];   // m: the row's (all its lanes); l: this lane's positions
-    int ev[MT];
+    // m + ev: what the row's scores are taken relative to (all its lanes); l: this lane's positions
+    float m[MT], l[MT], ev[MT];
   };
 
   // 16-byte chunk c of V row r (32 rows of HD 16-bit values) in LDS: the four rows of a
@@ -451,7 +460,7 @@ struct RowsTile {
       for (int x = 0; x < NC; ++x) y.acc[i][x] = f32x4{0, 0, 0, 0};
       y.m[i] = -INFINITY;
       y.l[i] = 0.0f;
-      y.ev[i] = -1000;
+      y.ev[i] = kExps ? kLeastExp : 0.0f;
     }
     char* const vlds = arena + wave * WB;
     if constexpr (MT > 1) __syncthreads();   // (Q of a pair of tiles leaves no registers for V)
@@ -515,26 +524,9 @@ struct RowsTile {
         float mx = s[i][0][0];
 #pragma unroll
         for (int x = 1; x < 8; ++x) mx = fmaxf(mx, s[i][x >> 2][x & 3]);
-        float alpha = 1.0f;
-        bool moved = false;
-        if (__builtin_amdgcn_ballot_w64(mx > y.m[i] + 8.0f) != 0) {
-          mx = fmaxf(mx, __shfl_xor(mx, 16));
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float mn = fmaxf(y.m[i], mx);
-          alpha = mn == -INFINITY ? 1.0f : exp2_fast(y.m[i] - mn);
-          y.m[i] = mn;
-          y.l[i] *= alpha;
-          moved = true;
-        }
-        const float mu = y.m[i] == -INFINITY ? 0.0f : y.m[i];
-        float p[8];
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          p[x] = exp2_fast(s[i][x >> 2][x & 3] - mu);
-          y.l[i] += p[x];
-        }
+        float w[8];
+        float big = kLeastExp;
         if constexpr (kCodes) {
-          float w[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) w[x] = vs[x];
           if (hides) {   // (a hidden token's scale may be NaN)
@@ -542,25 +534,34 @@ struct RowsTile {
             for (int x = 0; x < 8; ++x) w[x] = (x & 3) < lim[x >> 2] ? vs[x] : 0.0f;
           }
           if constexpr (kExps) {
-            // f16 has five exponent bits: the scales enter relative to a power of two just above
-            // the largest that the row has seen
-            float big = w[0];
+            float most = w[0];
 #pragma unroll
-            for (int x = 1; x < 8; ++x) big = fmaxf(big, w[x]);
-            int e = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000;
-            if (__builtin_amdgcn_ballot_w64(e > y.ev[i]) != 0) {
-              e = max(e, __shfl_xor(e, 16));
-              e = max(max(e, __shfl_xor(e, 32)), y.ev[i]);
-              alpha *= __builtin_ldexpf(1.0f, max(y.ev[i] - e, -300));
-              y.ev[i] = e;
-              moved = true;
-            }
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              w[x] = __builtin_ldexpf(w[x], y.ev[i] < -500 ? 0 : -y.ev[i]);
+            for (int x = 1; x < 8; ++x) most = fmaxf(most, w[x]);
+            big = scale_exp(most);
           }
+        }
+        float alpha = 1.0f;
+        bool moved = false;
+        if (__builtin_amdgcn_ballot_w64(mx > y.m[i] + 8.0f || (kExps && big > y.ev[i])) != 0) {
+          mx = fmaxf(mx, __shfl_xor(mx, 16));
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+          const float old = y.m[i] + y.ev[i];
+          y.m[i] = fmaxf(y.m[i], mx);
+          if constexpr (kExps) {
+            big = fmaxf(big, __shfl_xor(big, 16));
+            y.ev[i] = fmaxf(y.ev[i], fmaxf(big, __shfl_xor(big, 32)));
+          }
+          alpha = y.m[i] == -INFINITY ? 1.0f : exp2_fast(old - (y.m[i] + y.ev[i]));
+          y.l[i] *= alpha;
+          moved = true;
+        }
+        const float mu = y.m[i] == -INFINITY ? 0.0f : y.m[i] + y.ev[i];
+        float p[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) p[x] *= w[x];
+        for (int x = 0; x < 8; ++x) {
+          p[x] = exp2_fast(s[i][x >> 2][x & 3] - mu);
+          y.l[i] += p[x];
+          if constexpr (kCodes) p[x] *= w[x];
         }
         if (moved) {
 #pragma unroll
@@ -592,15 +593,10 @@ struct RowsTile {
       l += __shfl_xor(l, 32);
 #pragma unroll
       for (int x = 0; x < NC; ++x) {
-        if constexpr (kExps) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            y.acc[i][x][j] = y.ev[i] < -500 ? 0.0f : __builtin_ldexpf(y.acc[i][x][j], y.ev[i]);
-        }
         *reinterpret_cast<f32x4*>(wo + (16 * i + l16) * ORS + 16 * x + 4 * g) = y.acc[i][x];
       }
       if (g == 0) {
-        sm[wave][16 * i + l16] = y.m[i];
+        sm[wave][16 * i + l16] = y.m[i] + y.ev[i];
         sl[wave][16 * i + l16] = l;
       }
     }
@@ -789,6 +785,7 @@ struct ChunkTile {
   static_assert(HD == 64 || HD == 128, "chunk kernel head dim");
   static constexpr bool kCodes = cache_codes<CT>();
   static constexpr int ESZ = cache_size<CT>();
+  static constexpr bool kExps = kCodes && DT == kF16;   // (scale_exp)
   static constexpr int RB = HD * 2;                  // bytes of a row in LDS
   static constexpr int KBYTES = chunk::KB * RB;      // of a block's K (or V)
   static constexpr int CPR = HD * ESZ / 16;          // 16-byte pieces of a row in memory
@@ -799,6 +796,7 @@ struct ChunkTile {
   struct Lds {
     char kv[2][2 * KBYTES];
     float ks[2][chunk::KB], vs[2][chunk::KB];   // 0 where nothing is held
+    float big[2];                               // scale_exp of the largest of vs
     uint32_t there[2][4];                       // the pages of the block's four groups exist
     uint32_t odd[2];                            // the block with NaN or infinities in V
   };
@@ -900,8 +898,7 @@ attn_paged_chunk(AttnArgs a) {
   for (int i = 0; i < T::NDT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
-  int ev = -1000;   // f16 with codes: O is in units of 2^ev
+  float m = -INFINITY, l = 0.0f, ev = T::kExps ? kLeastExp : 0.0f;
   if (t < 2) sh.odd[t] = 0xffffffffu;
 
   // this thread's pieces of a block: rows xr, 16-byte pieces xc.  A wave's rows, from wr on, lie
@@ -973,6 +970,12 @@ attn_paged_chunk(AttnArgs a) {
     }
     if constexpr (T::kCodes) {
       if (t < 2 * KB) (t < KB ? sh.ks : sh.vs)[j & 1][t & 63] = st.scale;
+      if constexpr (T::kExps) {
+        if (wave == 1) {   // (its lanes hold all of vs)
+          const float most = wave_max(st.scale);
+          if (lane == 0) sh.big[j & 1] = scale_exp(most);
+        }
+      }
     }
     if (odd && (j + 1) * KB > tile_min) sh.odd[j & 1] = j;   // (any of them: one value)
   };
@@ -1035,16 +1038,33 @@ attn_paged_chunk(AttnArgs a) {
       for (int i = 1; i < 8; ++i) mx[q] = fmaxf(mx[q], s[q >> 1][8 * (q & 1) + i]);
     }
     const float top = pair_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * a.scale_log2;
+    float big = kLeastExp;
+    if constexpr (T::kExps) {
+      if (hides) {
+        float most = 0.0f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
+            most = fmaxf(most, at < lim ? sh.vs[j & 1][at + 4 * g] : 0.0f);
+          }
+        big = scale_exp(pair_max(most));
+      } else {
+        big = sh.big[j & 1];
+      }
+    }
     float alpha = 1.0f;
     bool moved = false;
-    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f) != 0) {
-      const float mn = fmaxf(m, top);
-      alpha = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
-      m = mn;
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || (T::kExps && big > ev)) != 0) {
+      const float old = m + ev;
+      m = fmaxf(m, top);
+      ev = T::kExps ? fmaxf(ev, big) : 0.0f;
+      alpha = m == -INFINITY ? 1.0f : exp2_fast(old - (m + ev));
       l *= alpha;
       moved = true;
     }
-    const float mu = m == -INFINITY ? 0.0f : m;
+    const float mu = m == -INFINITY ? 0.0f : m + ev;
     float l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -1054,30 +1074,6 @@ attn_paged_chunk(AttnArgs a) {
         (i & 1 ? l1 : l0) += s[kt][i];
       }
     l += l0 + l1;
-    if constexpr (T::kCodes) {
-      if constexpr (DT == kF16) {
-        // as in the rows' kernel: relative to the largest scale that the row has seen
-        float big = 0.0f;
-        if (hides) {
-#pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
-              big = fmaxf(big, at < lim ? sh.vs[j & 1][at + 4 * g] : 0.0f);
-            }
-          big = pair_max(big);
-        } else {
-          big = wave_max(sh.vs[j & 1][lane]);
-        }
-        const int e = max(ev, big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : -1000);
-        if (__builtin_amdgcn_ballot_w64(e > ev) != 0) {
-          alpha *= __builtin_ldexpf(1.0f, max(ev - e, -300));
-          ev = e;
-          moved = true;
-        }
-      }
-    }
     if (moved) {
 #pragma unroll
       for (int i = 0; i < T::NDT; ++i)
@@ -1090,10 +1086,9 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int at = 16 * sp + 8 * q;
-          f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][at + 4 * g]);
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][at + 4 * g]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if constexpr (DT == kF16) vs[i] = __builtin_ldexpf(vs[i], ev < -500 ? 0 : -ev);
             const int x = 8 * (sp & 1) + 4 * q + i;
             s[sp >> 1][x] *= vs[i];
             if (hides) s[sp >> 1][x] = at + i < lim ? s[sp >> 1][x] : 0.0f;   // (may be NaN)
@@ -1175,13 +1170,6 @@ attn_paged_chunk(AttnArgs a) {
   }
   if (!live_wave) return;
   l = pair_sum(l);
-  if constexpr (T::kCodes && DT == kF16) {
-#pragma unroll
-    for (int i = 0; i < T::NDT; ++i)
-#pragma unroll
-      for (int x = 0; x < 16; ++x)
-        acc[i][x] = ev < -500 ? 0.0f : __builtin_ldexpf(acc[i][x], ev);
-  }
   if (!live_row) return;
   const uint64_t at = (c.first + qi) * static_cast<uint64_t>(a.nh) + hq;
   if (whole) {
@@ -1210,7 +1198,7 @@ attn_paged_chunk(AttnArgs a) {
             f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
     if (g == 0) {
       rec_[HD] = l;
-      rec_[HD + 1] = m;
+      rec_[HD + 1] = m + ev;
     }
   }
 }

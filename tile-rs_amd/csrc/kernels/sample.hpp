@@ -1,8 +1,8 @@
 // Sampling of one token per row of logits: temperature, top-k, top-p, min-p, from a given
-// random number.  Bound by the row's bytes; the passes after the first read the caches.
+// random number.
 //
-//   w_i = exp((x_i - x_max) / T), held as whole numbers of 2^-31, so that masses are exact in
-//   64 bits and no order of summation shows.
+//   w_i = exp((x_i - x_max) / T) in f32, held as a whole number of 2^-40, so that masses are
+//   exact in 64 bits and no order of summation shows.
 //
 // The kept set is a prefix of the order (x falling, then index rising), so each limit is a cut:
 // a (key, index) pair, the last one kept, with `key` the order-preserving whole number of x.  A
@@ -13,6 +13,9 @@
 //
 // The token is then the first index whose mass with the lower ones' exceeds u times the kept
 // mass: the row is divided among the waves, and the share that holds the place is divided again.
+//
+// One workgroup of 16 waves per row.  Rows of up to 16 vectors of 16 bytes per thread stay in
+// registers between the passes, longer ones are read again (from the caches).
 #pragma once
 
 #include "common.hpp"
@@ -22,55 +25,141 @@ namespace smp {
 constexpr int NT = 1024, NW = NT / 64;
 constexpr int BINS = 2048;
 constexpr int CAP = 2048;       // members that are ranked in LDS
-constexpr float kLowest = 33.0f;   // 2^-33 rounds to no step of 2^-31
-constexpr uint32_t kOne = 1u << 31;
+constexpr float kLowest = 42.0f;   // 2^-42 rounds to no step of 2^-40
+constexpr uint64_t kOne = 1ull << 40;
+
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
+  return static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(v >> 32), o)) << 32 |
+         __shfl_xor(static_cast<uint32_t>(v), o);
+}
 
 struct Pair {   // a place in the order: larger key first, then lower index
   uint32_t key, idx;
 };
-__device__ __forceinline__ bool upto(uint32_t key, uint32_t idx, Pair cut) {
-  return key > cut.key || (key == cut.key && idx <= cut.idx);
-}
-
 __device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);   // (-0 is 0)
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
 
-// Row of logits; NaN counts as -infinity, and -0 as 0.
+// A row of logits.  NaN counts as -infinity: no comparison below takes it for anything else.
 template <int DT>
 struct Row {
+  static constexpr uint32_t E = Vec16<DT>::kElems;
   const void* p;
+  uint32_t vocab;
   __device__ __forceinline__ float operator[](uint32_t i) const {
-    float x;
-    if constexpr (DT == kF32) x = static_cast<const float*>(p)[i];
-    else x = u16_to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
-    return x != x ? -INFINITY : x + 0.0f;
+    if constexpr (DT == kF32) return static_cast<const float*>(p)[i];
+    else return u16_to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
+  }
+};
+
+// The row by aligned 16-byte blocks: block k holds elements k E - off + (0 .. E-1), those outside
+// the row as -infinity.  Wave w has the blocks [w per, (w + 1) per).  NV: blocks of a thread that
+// stay in registers; 0: every pass reads them.
+template <int DT, int NV>
+struct Blocks {
+  static constexpr uint32_t E = Row<DT>::E;
+  Row<DT> row;
+  const char* base;          // of block 0
+  uint32_t off, count, per;
+  const u32x4* edge;
+  u32x4 held[NV > 0 ? NV : 1];
+
+  // edges: LDS for the row's first and last block, which may not be whole.
+  __device__ __forceinline__ void init(const Row<DT>& r, u32x4* edges) {
+    row = r;
+    edge = edges;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(r.p);
+    off = static_cast<uint32_t>(at & 15u) / (16 / E);
+    base = reinterpret_cast<const char*>(at & ~uintptr_t{15});
+    count = (off + r.vocab + E - 1) / E;
+    per = NV > 0 ? 64u * NV : ((count + NW * 64 - 1) / (NW * 64)) * 64u;
+    if (threadIdx.x < 2 * E) {
+      const uint32_t k = threadIdx.x < E ? 0 : count - 1;
+      const int32_t i = static_cast<int32_t>(k * E - off + threadIdx.x % E);
+      const bool in = i >= 0 && i < static_cast<int32_t>(r.vocab);
+      if constexpr (DT == kF32)
+        reinterpret_cast<float*>(edges)[threadIdx.x] =
+            in ? static_cast<const float*>(r.p)[i] : -INFINITY;
+      else
+        reinterpret_cast<uint16_t*>(edges)[threadIdx.x] =
+            in ? static_cast<const uint16_t*>(r.p)[i] : static_cast<uint16_t>(kNone);
+    }
+    __syncthreads();
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) held[j] = load(first() + 64 * j);
+    }
+  }
+  __device__ __forceinline__ uint32_t first() const {
+    return (threadIdx.x >> 6) * per + (threadIdx.x & 63u);
+  }
+  static constexpr uint32_t kNone =   // -infinities
+      DT == kF32 ? 0xff800000u : DT == kBF16 ? 0xff80ff80u : 0xfc00fc00u;
+  __device__ __forceinline__ u32x4 load(uint32_t k) const {
+    u32x4 v = {kNone, kNone, kNone, kNone};
+    if (k > 0 && k + 1 < count) v = ldg128(base + 16ull * k);
+    else if (k < count) v = edge[k == 0 ? 0 : 1];
+    return v;
+  }
+  // f(index, logit) of every element of this thread (and -infinities outside the row).
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    auto block = [&](u32x4 v, uint32_t k) {
+      float x[E];
+      unpack16<DT>(v, x);
+#pragma unroll
+      for (int e = 0; e < static_cast<int>(E); ++e) f(k * E - off + e, x[e]);
+    };
+    if constexpr (NV > 0) {
+      // What a pass makes of the row is not kept for the next one (there are no registers for
+      // that): each works on copies that the compiler cannot tell from other values.
+      uint32_t k = first();
+      asm volatile("" : "+v"(k));
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        u32x4 v = held[j];
+        asm volatile("" : "+v"(v));
+        block(v, k + 64 * j);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      const uint32_t end = min(count, ((threadIdx.x >> 6) + 1) * per);
+      for (uint32_t k = first(); k < end; k += 64 * 4) {
+        u32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = load(k + 64 * j < end ? k + 64 * j : count);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) block(v[j], k + 64 * j);
+      }
+    }
   }
 };
 
 struct Weigher {
   float top, c_hi, c_lo;   // log2(e) / T as the sum of two floats
-  __device__ __forceinline__ uint32_t operator()(float x) const {
-    if (x == top) return kOne;   // (infinities too)
+  __device__ __forceinline__ float weight(float x) const {
     const float d = x - top;
-    if (!(d > -INFINITY)) return 0;
     const float y = d * c_hi;
-    if (y < -kLowest) return 0;
-    const float y_lo = __builtin_fmaf(d, c_hi, -y) + d * c_lo;
+    const float y_lo = __builtin_fmaf(d, c_lo, __builtin_fmaf(d, c_hi, -y));
     const float e = exp2_fast(y);
-    return static_cast<uint32_t>(
-        __builtin_rintf(__builtin_fmaf(e * y_lo, 0.69314718f, e) * static_cast<float>(kOne)));
+    const float w = __builtin_fmaf(e * y_lo, 0.69314718f, e);
+    // (x = top = infinity; differences of -infinity and NaN)
+    return x == top ? 1.0f : y > -kLowest ? w : 0.0f;
   }
+  // In steps of 2^-40: the fraction bits of 2^12 + w, to nearest even.
+  static __device__ __forceinline__ uint64_t steps(float w) {
+    return __builtin_bit_cast(uint64_t, static_cast<double>(w) + 4096.0) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ uint64_t operator()(float x) const { return steps(weight(x)); }
 };
 
 __device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t lo = __shfl_xor(static_cast<uint32_t>(v), o);
-    const uint32_t hi = __shfl_xor(static_cast<uint32_t>(v >> 32), o);
-    v += static_cast<uint64_t>(hi) << 32 | lo;
-  }
+  for (int o = 1; o < 64; o <<= 1) v += shfl_xor64(v, o);
   return v;
 }
 __device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {
@@ -97,14 +186,13 @@ struct Shared {
   uint32_t count[BINS];
   unsigned long long mass[BINS];
   uint64_t member[CAP];    // (key, ~index): larger comes first
-  uint32_t weight[CAP];
+  uint64_t weight[CAP];
   uint64_t wave_a[NW], wave_b[NW];
   float wave_f[NW];
   uint32_t members;
   uint32_t bin;
   uint64_t above_n, above_m, found, found_m;
-  uint32_t in_bin;
-  uint64_t lo, hi;
+  uint32_t in_bin, in_bin_first;
 };
 
 // The last bin that still holds a kept token: the first whose following bin the goal does not
@@ -144,66 +232,71 @@ __device__ __forceinline__ void find_bin(Shared& sh, const Goal& goal, uint64_t 
   __syncthreads();
 }
 
-template <int DT>
+template <int DT, int NV>
 struct Sampler {
-  Row<DT> row;
-  uint32_t vocab;
+  const Blocks<DT, NV>& row;
   Weigher weigh;
   float bin_scale;
   Shared& sh;
 
+  // BINS - 1: without weight (NaN and -infinity among them), which no pass counts
   __device__ __forceinline__ uint32_t bin_of(float x) const {
-    const float d = (weigh.top - x) * bin_scale;
-    return d < static_cast<float>(BINS - 1) ? static_cast<uint32_t>(d) : BINS - 1;
+    const float d = (weigh.top - x) * bin_scale;   // (x = top = infinity: NaN)
+    return x == weigh.top ? 0u : d < static_cast<float>(BINS - 1) ? static_cast<uint32_t>(d)
+                                                                  : BINS - 1;
   }
-
-  // Counts and masses of all tokens by bins of x.
-  __device__ __forceinline__ void histogram() {
-    const int t = threadIdx.x;
-    for (int i = t; i < BINS; i += NT) {
+  static __device__ __forceinline__ uint64_t place(float x, uint32_t i) {
+    return static_cast<uint64_t>(order_key(x)) << 32 | (0xffffffffu - i);
+  }
+  __device__ __forceinline__ void clear() const {
+    for (int i = threadIdx.x; i < BINS; i += NT) {
       sh.count[i] = 0;
       sh.mass[i] = 0;
     }
     __syncthreads();
-    for (uint32_t i = t; i < vocab; i += NT) {
-      const float x = row[i];
-      if (x == -INFINITY) continue;
-      const uint32_t b = x == weigh.top ? 0u : bin_of(x);
-      atomicAdd(&sh.count[b], 1u);
-      const uint32_t w = weigh(x);
-      if (w) atomicAdd(&sh.mass[b], static_cast<unsigned long long>(w));
-    }
+  }
+
+  // Counts and masses of all tokens with weight by bins of x.
+  __device__ __forceinline__ void histogram() const {
+    clear();
+    row.each([&](uint32_t, float x) {
+      const uint32_t b = bin_of(x);
+      const uint64_t w = weigh(x);
+      if (b < BINS - 1) {
+        atomicAdd(&sh.count[b], 1u);
+        atomicAdd(&sh.mass[b], static_cast<unsigned long long>(w));
+      }
+    });
     __syncthreads();
   }
 
-  // The goal's cut among the tokens up to `cut`; sum: the mass up to the new cut.  The bins are
-  // those of histogram(), whole rows (a goal is met at or before `cut` if it was chosen so).
-  __device__ __forceinline__ Pair select(const Goal& goal, Pair cut, uint64_t* sum) {
+  // The goal's cut; sum: the mass up to it.  The bins are those of histogram().
+  __device__ __forceinline__ Pair select(const Goal& goal, uint64_t* sum) const {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     find_bin(sh, goal, 0, 0);
     // every token is wanted, or the cut is among those without weight
-    if (sh.bin >= BINS - 1) return cut;
+    if (sh.bin >= BINS) return Pair{0, 0xffffffffu};
     const uint32_t first_bin = sh.bin;
-    uint64_t lo = 0, hi = ~0ull;   // members' (key, ~index)
+    uint64_t lo = 0, hi = ~0ull;   // the members' places
+    auto members = [&](auto&& f) {
+      row.each([&](uint32_t i, float x) {
+        if (bin_of(x) != first_bin) return;
+        const uint64_t v = place(x, i);
+        if (v >= lo && v <= hi) f(v, x);
+      });
+    };
+    if (t == 0) sh.in_bin_first = sh.in_bin;
     while (sh.in_bin > CAP) {
       // divide the members again, evenly between the least and the largest of them
       uint64_t a = ~0ull, b = 0;
-      for (uint32_t i = t; i < vocab; i += NT) {
-        const float x = row[i];
-        if (x == -INFINITY || (x == weigh.top ? 0u : bin_of(x)) != first_bin) continue;
-        const uint64_t v = static_cast<uint64_t>(order_key(x)) << 32 | (0xffffffffu - i);
-        if (v < lo || v > hi) continue;
+      members([&](uint64_t v, float) {
         a = min(a, v);
         b = max(b, v);
-      }
+      });
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t a2 = static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(a >> 32), o)) << 32 |
-                            __shfl_xor(static_cast<uint32_t>(a), o);
-        const uint64_t b2 = static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(b >> 32), o)) << 32 |
-                            __shfl_xor(static_cast<uint32_t>(b), o);
-        a = min(a, a2);
-        b = max(b, b2);
+        a = min(a, shfl_xor64(a, o));
+        b = max(b, shfl_xor64(b, o));
       }
       if (lane == 0) {
         sh.wave_a[wave] = a;
@@ -219,24 +312,15 @@ struct Sampler {
       hi = b;
       int shift = 0;   // bin 0 has the largest
       while (((hi - lo) >> shift) >= BINS) ++shift;
-      for (int i = t; i < BINS; i += NT) {
-        sh.count[i] = 0;
-        sh.mass[i] = 0;
-      }
-      __syncthreads();
-      for (uint32_t i = t; i < vocab; i += NT) {
-        const float x = row[i];
-        if (x == -INFINITY || (x == weigh.top ? 0u : bin_of(x)) != first_bin) continue;
-        const uint64_t v = static_cast<uint64_t>(order_key(x)) << 32 | (0xffffffffu - i);
-        if (v < lo || v > hi) continue;
+      clear();
+      members([&](uint64_t v, float x) {
         const uint32_t q = static_cast<uint32_t>((hi - v) >> shift);
         atomicAdd(&sh.count[q], 1u);
         atomicAdd(&sh.mass[q], static_cast<unsigned long long>(weigh(x)));
-      }
+      });
       __syncthreads();
       find_bin(sh, goal, base_n, base_m);
-      const uint64_t q = sh.bin;
-      const uint64_t top = hi - (q << shift);
+      const uint64_t top = hi - (static_cast<uint64_t>(sh.bin) << shift);
       const uint64_t width = (1ull << shift) - 1;
       lo = top - lo > width ? top - width : lo;
       hi = top;
@@ -244,17 +328,13 @@ struct Sampler {
     // the members, in any order; each is ranked by a walk over the others
     if (t == 0) sh.members = 0;
     __syncthreads();
-    for (uint32_t i = t; i < vocab; i += NT) {
-      const float x = row[i];
-      if (x == -INFINITY || (x == weigh.top ? 0u : bin_of(x)) != first_bin) continue;
-      const uint64_t v = static_cast<uint64_t>(order_key(x)) << 32 | (0xffffffffu - i);
-      if (v < lo || v > hi) continue;
+    members([&](uint64_t v, float x) {
       const uint32_t at = atomicAdd(&sh.members, 1u);
       if (at < CAP) {
         sh.member[at] = v;
         sh.weight[at] = weigh(x);
       }
-    }
+    });
     __syncthreads();
     const uint32_t n = min(sh.members, static_cast<uint32_t>(CAP));
     for (uint32_t i = t; i < n; i += NT) {
@@ -263,7 +343,7 @@ struct Sampler {
       for (uint32_t j = 0; j < n; ++j) {
         const bool before = sh.member[j] > v;
         bn += before;
-        bm += before ? sh.weight[j] : 0u;
+        bm += before ? sh.weight[j] : 0ull;
       }
       if (goal.wants(bn, bm) && !goal.wants(bn + 1, bm + sh.weight[i])) {
         sh.found = v;
@@ -279,7 +359,7 @@ struct Sampler {
 };
 
 // One workgroup per row.
-template <int DT>
+template <int DT, int NV>
 __global__ void __launch_bounds__(NT)
 sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint32_t vocab,
             uint64_t stride, const float* __restrict__ uniform,
@@ -291,50 +371,41 @@ sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const float temp = temperature ? temperature[r] : 1.0f;
   const int32_t k = top_k ? top_k[r] : 0;
-  const float p = top_p ? top_p[r] : 1.0f, mp = min_p ? min_p[r] : 0.0f;
-  const Row<DT> row{static_cast<const char*>(logits) + r * stride * (DT == kF32 ? 4 : 2)};
+  const float p = top_p ? top_p[r] : 1.0f, mp = fmaxf(min_p ? min_p[r] : 0.0f, 0.0f);   // (no NaN)
+  const float u = uniform[r];
+  const Row<DT> row{static_cast<const char*>(logits) + r * stride * (DT == kF32 ? 4 : 2), vocab};
+  Blocks<DT, NV> blocks;
+  __shared__ u32x4 edges[2];
+  blocks.init(row, edges);
 
-  // the largest logit and its lowest index
   float top = -INFINITY;
-  uint32_t at = 0xffffffffu;
-  for (uint32_t i = t; i < vocab; i += NT) {
-    const float x = row[i];
-    if (x > top) {
-      top = x;
-      at = i;
-    }
-  }
-  {
-    uint64_t v = static_cast<uint64_t>(order_key(top)) << 32 | (0xffffffffu - at);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint64_t v2 = static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(v >> 32), o)) << 32 |
-                          __shfl_xor(static_cast<uint32_t>(v), o);
-      v = max(v, v2);
-    }
-    if (lane == 0) sh.wave_a[wave] = v;
-    __syncthreads();
-    for (int i = 0; i < NW; ++i) v = max(v, sh.wave_a[i]);
-    const uint32_t key = static_cast<uint32_t>(v >> 32);
-    top = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-    at = 0xffffffffu - static_cast<uint32_t>(v);
-    __syncthreads();
-  }
+  blocks.each([&](uint32_t, float x) { top = fmaxf(top, x); });
+  top = wave_max(top);
+  if (lane == 0) sh.wave_f[wave] = top;
+  __syncthreads();
+  for (int i = 0; i < NW; ++i) top = fmaxf(top, sh.wave_f[i]);
   if (top == -INFINITY) {
     if (t == 0) tokens[r] = -1;
     return;
   }
-  // one token is kept (or asked for): the first
+  // one token is kept (or asked for): the first of the largest
   if (!(temp > 0.0f) || k == 1 || p <= 0.0f || mp > 1.0f) {
+    uint32_t at = 0xffffffffu;
+    blocks.each([&](uint32_t i, float x) { at = x == top ? min(at, i) : at; });
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) at = min(at, __shfl_xor(at, o));
+    if (lane == 0) sh.wave_a[wave] = at;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) at = min(at, static_cast<uint32_t>(sh.wave_a[i]));
     if (t == 0) tokens[r] = static_cast<int32_t>(at);
     return;
   }
-  const double c = 1.4426950408889634 / static_cast<double>(temp);
+  const double c = min(1.4426950408889634 / static_cast<double>(temp), 3.0e38);
   Weigher weigh;
   weigh.top = top;
-  weigh.c_hi = static_cast<float>(min(c, 3.0e38));
-  weigh.c_lo = static_cast<float>(min(c, 3.0e38) - static_cast<double>(weigh.c_hi));
-  Sampler<DT> s{row, vocab, weigh, weigh.c_hi * (static_cast<float>(BINS - 1) / kLowest), sh};
+  weigh.c_hi = static_cast<float>(c);
+  weigh.c_lo = static_cast<float>(c - static_cast<double>(weigh.c_hi));
+  const Sampler<DT, NV> s{blocks, weigh, weigh.c_hi * (static_cast<float>(BINS - 1) / kLowest), sh};
 
   Pair cut{0, 0xffffffffu};
   const bool cut_k = k > 0 && static_cast<uint32_t>(k) < vocab, cut_p = p < 1.0f;
@@ -342,75 +413,90 @@ sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
     s.histogram();
     uint64_t whole = 0;
     if (cut_p) {   // all the row's mass, unless top-k leaves less
-      uint64_t m = wave_sum64(sh.mass[2 * t] + sh.mass[2 * t + 1]);
+      const uint64_t m = wave_sum64(sh.mass[2 * t] + sh.mass[2 * t + 1]);
       if (lane == 0) sh.wave_a[wave] = m;
       __syncthreads();
       for (int i = 0; i < NW; ++i) whole += sh.wave_a[i];
       __syncthreads();
     }
+    bool fresh = true;   // the bins are the histogram's
     if (cut_k) {
-      cut = s.select(Goal{false, static_cast<uint64_t>(k), 0.0}, cut, &whole);
+      cut = s.select(Goal{false, static_cast<uint64_t>(k), 0.0}, &whole);
+      fresh = sh.bin >= BINS || sh.in_bin_first <= CAP;
       __syncthreads();
     }
     if (cut_p) {
-      if (cut_k) s.histogram();   // (a division may have used the bins)
+      if (!fresh) s.histogram();
       uint64_t sum;
       const Pair by_p =
-          s.select(Goal{true, 0, static_cast<double>(p) * static_cast<double>(whole)}, cut, &sum);
-      if (!upto(by_p.key, by_p.idx, cut)) {
-        // rounding put the mass cut behind the other: the other holds
-      } else {
-        cut = by_p;
-      }
+          s.select(Goal{true, 0, static_cast<double>(p) * static_cast<double>(whole)}, &sum);
+      // the stricter of the two
+      if (by_p.key > cut.key || (by_p.key == cut.key && by_p.idx < cut.idx)) cut = by_p;
       __syncthreads();
     }
   }
 
-  // kept mass of [a, b) by waves; then the place, in the share that holds it
-  auto kept = [&](uint32_t i) -> uint32_t {
-    const float x = row[i];
-    if (x == -INFINITY || !upto(order_key(x), i, cut)) return 0;
-    const uint32_t w = weigh(x);
-    return static_cast<float>(w) * (1.0f / static_cast<float>(kOne)) >= mp || !(mp > 0.0f) ? w : 0u;
+  // kept mass by waves; then the place, in the share that holds it
+  const bool all_kept = cut.key == 0 && mp == 0.0f;
+  const float cut_x = cut.key == 0 ? -INFINITY : key_value(cut.key);
+  auto kept = [&](uint32_t i, float x) -> uint64_t {
+    const float w = weigh.weight(x);
+    const bool in = (w >= mp) & ((x > cut_x) | ((x == cut_x) & (i <= cut.idx)));
+    return Weigher::steps(in ? w : 0.0f);
   };
+  uint64_t m = 0;
+  if (all_kept)
+    blocks.each([&](uint32_t, float x) { m += weigh(x); });
+  else
+    blocks.each([&](uint32_t i, float x) {
+      // (a cut leaves few: most waves skip most weights)
+      if (__builtin_amdgcn_ballot_w64(x >= cut_x) != 0) m += kept(i, x);
+    });
   uint32_t a = 0, b = vocab;
   uint64_t before = 0;   // mass below a
   double target = 0.0;
-  bool first = true;
-  while (true) {
-    const uint32_t share = (b - a + NW - 1) / NW;
-    const uint32_t wa = min(b, a + wave * share), wb = min(b, wa + share);
-    uint64_t m = 0;
-    for (uint32_t i = wa + lane; i < wb; i += 64) m += kept(i);
+  {
     m = wave_sum64(m);
     if (lane == 0) sh.wave_a[wave] = m;
     __syncthreads();
-    if (first) {
-      uint64_t all = 0;
-      for (int i = 0; i < NW; ++i) all += sh.wave_a[i];
-      const float u = uniform[r];
-      target = min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0,
-                   static_cast<double>(all) - 0.5);
-      first = false;
-    }
+    uint64_t all = 0;
+    for (int i = 0; i < NW; ++i) all += sh.wave_a[i];
+    target = min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0,
+                 static_cast<double>(all) - 0.5);
     int w = 0;
-    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target) {
-      before += sh.wave_a[w];
-      ++w;
-    }
+    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
+      before += sh.wave_a[w++];
+    __syncthreads();
+    // the wave's blocks as elements
+    const uint64_t e0 = static_cast<uint64_t>(w) * blocks.per * Row<DT>::E;
+    const uint64_t e1 = e0 + static_cast<uint64_t>(blocks.per) * Row<DT>::E;
+    a = static_cast<uint32_t>(e0 > blocks.off ? e0 - blocks.off : 0);
+    b = static_cast<uint32_t>(min(static_cast<uint64_t>(vocab), e1 - blocks.off));
+  }
+  while (b - a > 64) {
+    const uint32_t share = (b - a + NW - 1) / NW;
+    const uint32_t wa = min(b, a + wave * share), wb = min(b, wa + share);
+    m = 0;
+#pragma unroll 8
+    for (uint32_t i = wa + lane; i < wb; i += 64) m += kept(i, row[i]);
+    m = wave_sum64(m);
+    if (lane == 0) sh.wave_a[wave] = m;
+    __syncthreads();
+    int w = 0;
+    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
+      before += sh.wave_a[w++];
     __syncthreads();
     const uint32_t na = min(b, a + w * share);
     b = min(b, na + share);
     a = na;
-    if (b - a <= 64) break;
   }
   if (wave == 0) {
     const uint32_t i = a + lane;
-    const uint64_t m = wave_scan64(i < b ? kept(i) : 0u, lane);
+    m = wave_scan64(i < b ? kept(i, row[i]) : 0ull, lane);
     const uint64_t over =
         __builtin_amdgcn_ballot_w64(i < b && static_cast<double>(before + m) > target);
     if (lane == 0)
-      tokens[r] = static_cast<int32_t>(over ? a + __builtin_ctzll(over) : at);
+      tokens[r] = static_cast<int32_t>(a + (over ? __builtin_ctzll(over) : 0));
   }
 }
 

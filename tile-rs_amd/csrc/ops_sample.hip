@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels/sample.hpp"
 #include "ops_common.hpp"
@@ -12,12 +13,24 @@ using namespace th::ops;
 
 namespace {
 
+// Rows of up to 16 vectors per thread stay in registers; the least that holds them.
 template <int DT>
 int sample_go(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab, uint64_t stride,
               const float* uniform, const float* temperature, const int32_t* top_k,
               const float* top_p, const float* min_p, hipStream_t s) {
-  hipLaunchKernelGGL((th::smp::sample_rows<DT>), dim3(rows), dim3(th::smp::NT), 0, s, logits,
-                     tokens, vocab, stride, uniform, temperature, top_k, top_p, min_p);
+  constexpr uint32_t E = th::smp::Row<DT>::E;
+  const uint64_t blocks = (static_cast<uint64_t>(vocab) + E - 1 + E - 1) / E;   // at any alignment
+  auto go = [&](auto nv) {
+    hipLaunchKernelGGL((th::smp::sample_rows<DT, nv.value>), dim3(rows), dim3(th::smp::NT), 0, s,
+                       logits, tokens, vocab, stride, uniform, temperature, top_k, top_p, min_p);
+  };
+  using std::integral_constant;
+  if (blocks <= 1024 * 2) go(integral_constant<int, 2>{});
+  else if (blocks <= 1024 * 4) go(integral_constant<int, 4>{});
+  else if (blocks <= 1024 * 8) go(integral_constant<int, 8>{});
+  else if (blocks <= 1024 * 13) go(integral_constant<int, 13>{});
+  else if (blocks <= 1024 * 16) go(integral_constant<int, 16>{});
+  else go(integral_constant<int, 0>{});
   return launch_status("sample launch");
 }
 
