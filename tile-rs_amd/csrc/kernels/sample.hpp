@@ -50,10 +50,6 @@ struct Row {
   static constexpr uint32_t E = Vec16<DT>::kElems;
   const void* p;
   uint32_t vocab;
-  __device__ __forceinline__ float operator[](uint32_t i) const {
-    if constexpr (DT == kF32) return static_cast<const float*>(p)[i];
-    else return u16_to_f32<DT>(static_cast<const uint16_t*>(p)[i]);
-  }
 };
 
 // The row by aligned 16-byte blocks: block k holds elements k E - off + (0 .. E-1), those outside
@@ -94,6 +90,8 @@ struct Blocks {
       for (int j = 0; j < NV; ++j) held[j] = load(first() + 64 * j);
     }
   }
+  __device__ __forceinline__ uint32_t index(uint32_t k) const { return k * E - off; }
+  static __device__ __forceinline__ void unpack(u32x4 v, float (&x)[E]) { unpack16<DT>(v, x); }
   __device__ __forceinline__ uint32_t first() const {
     return (threadIdx.x >> 6) * per + (threadIdx.x & 63u);
   }
@@ -112,7 +110,7 @@ struct Blocks {
       float x[E];
       unpack16<DT>(v, x);
 #pragma unroll
-      for (int e = 0; e < static_cast<int>(E); ++e) f(k * E - off + e, x[e]);
+      for (int e = 0; e < static_cast<int>(E); ++e) f(index(k) + e, x[e]);
     };
     if constexpr (NV > 0) {
       // What a pass makes of the row is not kept for the next one (there are no registers for
@@ -141,6 +139,11 @@ struct Blocks {
 
 struct Weigher {
   float top, c_hi, c_lo;   // log2(e) / T as the sum of two floats
+  static __device__ __forceinline__ Weigher make(float top, float temp) {
+    const double c = min(1.4426950408889634 / static_cast<double>(temp), 3.0e38);
+    const float hi = static_cast<float>(c);
+    return Weigher{top, hi, static_cast<float>(c - static_cast<double>(hi))};
+  }
   __device__ __forceinline__ float weight(float x) const {
     const float d = x - top;
     const float y = d * c_hi;
@@ -358,6 +361,61 @@ struct Sampler {
   }
 };
 
+// The first element of blocks [k0, k1) at which the mass from `before` on exceeds `target`, which
+// lies in them.  A long range is divided among the waves, and the share that holds the place
+// divided again, down to a block per thread.  kept(index, logit): an element's mass.
+template <class B, class F>
+__device__ __forceinline__ void find_place(Shared& sh, const B& row, uint32_t k0, uint32_t k1,
+                                           uint64_t before, double target, F&& kept,
+                                           int32_t* token) {
+  constexpr uint32_t E = B::E;
+  const int t = threadIdx.x, lane = t & 63;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  float x[E];
+  auto elements = [&](uint32_t k) { B::unpack(row.load(k), x); };
+  while (k1 - k0 > NT) {
+    const uint32_t share = (k1 - k0 + NW - 1) / NW;
+    const uint32_t wa = min(k1, k0 + wave * share), wb = min(k1, wa + share);
+    uint64_t m = 0;
+#pragma unroll 2
+    for (uint32_t k = wa + lane; k < wb; k += 64) {
+      elements(k);
+#pragma unroll
+      for (int e = 0; e < static_cast<int>(E); ++e) m += kept(row.index(k) + e, x[e]);
+    }
+    m = wave_sum64(m);
+    if (lane == 0) sh.wave_a[wave] = m;
+    __syncthreads();
+    uint32_t w = 0;
+    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
+      before += sh.wave_a[w++];
+    __syncthreads();
+    k0 = min(k1, k0 + w * share);
+    k1 = min(k1, k0 + share);
+  }
+  const uint32_t k = k0 + t;
+  elements(k < k1 ? k : row.count);
+  uint64_t m = 0;
+#pragma unroll
+  for (int e = 0; e < static_cast<int>(E); ++e) m += kept(row.index(k) + e, x[e]);
+  const uint64_t upto = wave_scan64(m, lane);
+  if (lane == 63) sh.wave_a[wave] = upto;
+  __syncthreads();
+  for (uint32_t w = 0; w < wave; ++w) before += sh.wave_a[w];
+  before += upto - m;
+  // one thread's block holds the place
+  if (m != 0 && static_cast<double>(before) <= target &&
+      static_cast<double>(before + m) > target) {
+    uint32_t at = 0;
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(E); ++e) {
+      before += kept(row.index(k) + e, x[e]);
+      at += static_cast<double>(before) <= target;
+    }
+    *token = static_cast<int32_t>(row.index(k) + at);
+  }
+}
+
 // One workgroup per row.
 template <int DT, int NV>
 __global__ void __launch_bounds__(NT)
@@ -400,11 +458,7 @@ sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
     if (t == 0) tokens[r] = static_cast<int32_t>(at);
     return;
   }
-  const double c = min(1.4426950408889634 / static_cast<double>(temp), 3.0e38);
-  Weigher weigh;
-  weigh.top = top;
-  weigh.c_hi = static_cast<float>(c);
-  weigh.c_lo = static_cast<float>(c - static_cast<double>(weigh.c_hi));
+  const Weigher weigh = Weigher::make(top, temp);
   const Sampler<DT, NV> s{blocks, weigh, weigh.c_hi * (static_cast<float>(BINS - 1) / kLowest), sh};
 
   Pair cut{0, 0xffffffffu};
@@ -452,52 +506,159 @@ sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
       // (a cut leaves few: most waves skip most weights)
       if (__builtin_amdgcn_ballot_w64(x >= cut_x) != 0) m += kept(i, x);
     });
-  uint32_t a = 0, b = vocab;
-  uint64_t before = 0;   // mass below a
-  double target = 0.0;
-  {
-    m = wave_sum64(m);
-    if (lane == 0) sh.wave_a[wave] = m;
-    __syncthreads();
-    uint64_t all = 0;
-    for (int i = 0; i < NW; ++i) all += sh.wave_a[i];
-    target = min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0,
-                 static_cast<double>(all) - 0.5);
-    int w = 0;
-    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
-      before += sh.wave_a[w++];
-    __syncthreads();
-    // the wave's blocks as elements
-    const uint64_t e0 = static_cast<uint64_t>(w) * blocks.per * Row<DT>::E;
-    const uint64_t e1 = e0 + static_cast<uint64_t>(blocks.per) * Row<DT>::E;
-    a = static_cast<uint32_t>(e0 > blocks.off ? e0 - blocks.off : 0);
-    b = static_cast<uint32_t>(min(static_cast<uint64_t>(vocab), e1 - blocks.off));
+  m = wave_sum64(m);
+  if (lane == 0) sh.wave_a[wave] = m;
+  __syncthreads();
+  uint64_t all = 0, before = 0;
+  for (int i = 0; i < NW; ++i) all += sh.wave_a[i];
+  const double target = min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0,
+                            static_cast<double>(all) - 0.5);
+  uint32_t w = 0;
+  while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
+    before += sh.wave_a[w++];
+  __syncthreads();
+  find_place(sh, blocks, min(blocks.count, w * blocks.per),
+             min(blocks.count, (w + 1) * blocks.per), before, target, kept, tokens + r);
+}
+
+// ---- few long rows without limits: each over many workgroups -------------------------------
+//
+// A part is kPart blocks of a row; its weights are relative to its own largest logit, so that
+// one pass gives part and mass, and sample_pick brings them together in f64.  One row of 128256
+// takes a CU 25 us (14 cycles of vector ALU per logit), the two launches 10.
+constexpr uint32_t kPart = NT;
+struct PartSum {
+  float top;
+  uint32_t pad;
+  uint64_t mass;
+};
+template <int DT>
+__global__ void __launch_bounds__(256)
+sample_parts(const void* __restrict__ logits, PartSum* __restrict__ sums, uint32_t vocab,
+             uint64_t stride, const float* __restrict__ temperature, uint32_t parts) {
+  __shared__ u32x4 edges[2];
+  __shared__ float tops[4];
+  __shared__ uint64_t masses[4];
+  const uint32_t r = blockIdx.x / parts, part = blockIdx.x % parts;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const float temp = temperature ? temperature[r] : 1.0f;
+  Blocks<DT, 0> blocks;
+  blocks.init(Row<DT>{static_cast<const char*>(logits) + r * stride * (DT == kF32 ? 4 : 2), vocab},
+              edges);
+  constexpr int N = kPart / 256, E = Row<DT>::E;
+  u32x4 v[N];
+  float x[N][E], top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = blocks.load(part * kPart + 256 * j + t);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    unpack16<DT>(v[j], x[j]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = fmaxf(top, x[j][e]);
   }
-  while (b - a > 64) {
-    const uint32_t share = (b - a + NW - 1) / NW;
-    const uint32_t wa = min(b, a + wave * share), wb = min(b, wa + share);
-    m = 0;
-#pragma unroll 8
-    for (uint32_t i = wa + lane; i < wb; i += 64) m += kept(i, row[i]);
-    m = wave_sum64(m);
-    if (lane == 0) sh.wave_a[wave] = m;
-    __syncthreads();
-    int w = 0;
-    while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
-      before += sh.wave_a[w++];
-    __syncthreads();
-    const uint32_t na = min(b, a + w * share);
-    b = min(b, na + share);
-    a = na;
+  top = wave_max(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const Weigher weigh = Weigher::make(top, temp);
+  uint64_t m = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int e = 0; e < E; ++e) m += weigh(x[j][e]);
+  m = wave_sum64(m);
+  if (lane == 0) masses[wave] = m;
+  __syncthreads();
+  if (t == 0)
+    sums[static_cast<uint64_t>(r) * parts + part] =
+        PartSum{top, 0, top == -INFINITY ? 0 : masses[0] + masses[1] + masses[2] + masses[3]};
+}
+
+template <int DT>
+__global__ void __launch_bounds__(NT)
+sample_pick(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint32_t vocab,
+            uint64_t stride, const float* __restrict__ uniform,
+            const float* __restrict__ temperature, const PartSum* __restrict__ sums,
+            uint32_t parts) {
+  __shared__ Shared sh;
+  const uint32_t r = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 63;
+  const float temp = temperature ? temperature[r] : 1.0f, u = uniform[r];
+  __shared__ u32x4 edges[2];
+  Blocks<DT, 0> blocks;
+  blocks.init(Row<DT>{static_cast<const char*>(logits) + r * stride * (DT == kF32 ? 4 : 2), vocab},
+              edges);
+  sums += static_cast<uint64_t>(r) * parts;
+  float top = -INFINITY;
+  for (uint32_t i = lane; i < parts; i += 64) top = fmaxf(top, sums[i].top);
+  top = wave_max(top);
+  if (top == -INFINITY) {
+    if (t == 0) tokens[r] = -1;
+    return;
   }
-  if (wave == 0) {
-    const uint32_t i = a + lane;
-    m = wave_scan64(i < b ? kept(i, row[i]) : 0ull, lane);
-    const uint64_t over =
-        __builtin_amdgcn_ballot_w64(i < b && static_cast<double>(before + m) > target);
-    if (lane == 0)
-      tokens[r] = static_cast<int32_t>(a + (over ? __builtin_ctzll(over) : 0));
+  // Masses relative to the row's largest logit, summed 64 parts at a time in a fixed order; then
+  // the part that holds u.  Every wave does it on its own.
+  const bool greedy = !(temp > 0.0f);
+  const double c = greedy ? 0.0 : 1.4426950408889634 / static_cast<double>(temp);
+  auto factor = [&](float x) {
+    if (x == top) return 1.0;
+    return greedy || !(x > -INFINITY) ? 0.0 : exp2(max(-2000.0, (static_cast<double>(x) - top) * c));
+  };
+  double mass = 0.0, upto = 0.0;   // of this lane's part, and of the 64's up to it
+  auto sum64 = [&](uint32_t base) {
+    const uint32_t i = base + lane;
+    mass = i < parts ? static_cast<double>(sums[i].mass) * factor(sums[i].top) : 0.0;
+    upto = mass;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(upto, o);
+      if (lane >= o) upto += y;
+    }
+  };
+  double all = 0.0;
+  uint32_t base = 0;
+  for (; base < parts; base += 64) {
+    sum64(base);
+    all += __shfl(upto, 63);
   }
+  const double target =
+      greedy || !(u > 0.0f) ? 0.0 : min(static_cast<double>(u) * all, all * (1.0 - 0x1p-52));
+  double before = 0.0;
+  uint32_t part = 0;
+  for (base = 0; base < parts; base += 64) {
+    if (parts > 64) sum64(base);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(mass > 0.0 && before + upto > target);
+    if (in != 0) {
+      const int l = __builtin_ctzll(in);
+      part = base + l;
+      before += __shfl(upto - mass, l);
+      break;
+    }
+    before += __shfl(upto, 63);
+  }
+  const float part_top = sums[part].top;
+  const double f = factor(part_top);
+  const uint32_t k0 = part * kPart, k1 = min(blocks.count, k0 + kPart);
+  if (greedy) {
+    float x[Blocks<DT, 0>::E];
+    Blocks<DT, 0>::unpack(blocks.load(k0 + t), x);
+    uint32_t at = 0xffffffffu;
+#pragma unroll
+    for (int e = 0; e < static_cast<int>(Blocks<DT, 0>::E); ++e)
+      at = x[e] == top ? min(at, blocks.index(k0 + t) + e) : at;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) at = min(at, __shfl_xor(at, o));
+    if (lane == 0) sh.wave_a[t >> 6] = at;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) at = min(at, static_cast<uint32_t>(sh.wave_a[i]));
+    if (t == 0) tokens[r] = static_cast<int32_t>(at);
+    return;
+  }
+  const Weigher weigh = Weigher::make(part_top, temp);
+  const double local =
+      max(0.0, min((target - before) / f, static_cast<double>(sums[part].mass) - 0.5));
+  find_place(sh, blocks, k0, k1, 0, local, [&](uint32_t, float x) { return weigh(x); },
+             tokens + r);
 }
 
 }  // namespace smp

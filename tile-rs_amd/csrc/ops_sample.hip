@@ -24,6 +24,21 @@ int sample_go(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab
     hipLaunchKernelGGL((th::smp::sample_rows<DT, nv.value>), dim3(rows), dim3(th::smp::NT), 0, s,
                        logits, tokens, vocab, stride, uniform, temperature, top_k, top_p, min_p);
   };
+  // Without limits, and with too few rows for the CUs, long rows are divided; their sums go to
+  // the stream's scratch, which a captured stream does not offer.
+  const uint32_t parts = static_cast<uint32_t>((blocks + th::smp::kPart - 1) / th::smp::kPart);
+  if (!top_k && !top_p && !min_p && parts > 4 && 2ull * rows <= current_cu_count() &&
+      !stream_capturing(s)) {
+    void* sums = nullptr;
+    th::ScratchHold hold;
+    TH_TRY(th::stream_scratch(s, sizeof(th::smp::PartSum) * rows * parts, &sums, &hold));
+    auto* ps = static_cast<th::smp::PartSum*>(sums);
+    hipLaunchKernelGGL((th::smp::sample_parts<DT>), dim3(rows * parts), dim3(256), 0, s, logits, ps,
+                       vocab, stride, temperature, parts);
+    hipLaunchKernelGGL((th::smp::sample_pick<DT>), dim3(rows), dim3(th::smp::NT), 0, s, logits,
+                       tokens, vocab, stride, uniform, temperature, ps, parts);
+    return launch_status("sample launch");
+  }
   using std::integral_constant;
   if (blocks <= 1024 * 2) go(integral_constant<int, 2>{});
   else if (blocks <= 1024 * 4) go(integral_constant<int, 4>{});
