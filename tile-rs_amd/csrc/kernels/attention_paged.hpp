@@ -12,6 +12,8 @@
 #include "common.hpp"
 #include "kv_cache.hpp"
 
+#include <type_traits>
+
 namespace th {
 namespace pgd {
 
@@ -85,6 +87,20 @@ __device__ __forceinline__ u32x4 load_within(const void* p, uint32_t bytes, uint
 }
 // An offset that is past every range.
 constexpr uint32_t kPast = 0x7ffffff0u;
+
+// The table's entry for min(pos, end - 1), 1 <= end <= cap, unchecked (paged_checked): whatever is
+// done with it waits for the load.
+__device__ __forceinline__ int32_t wave_entry(const PagedSeqs& s, uint32_t b, uint32_t pos,
+                                              uint32_t end) {
+  typedef __attribute__((address_space(4))) const int32_t* scalar_ptr;
+  b = __builtin_amdgcn_readfirstlane(b);
+  pos = __builtin_amdgcn_readfirstlane(pos);
+  const uint64_t at = static_cast<uint64_t>(b) * s.max_pages + (min(pos, end - 1) >> s.shift);
+  return *(scalar_ptr)(reinterpret_cast<uintptr_t>(s.table + at));
+}
+__device__ __forceinline__ int32_t paged_checked(const PagedSeqs& s, int32_t id) {
+  return static_cast<uint32_t>(id) < s.num_pages ? id : -1;   // (num_pages is below 2^31)
+}
 
 // f16 probabilities times scales need not fit f16's five exponent bits.  So the scores of a row
 // are taken relative to its maximum plus the exponent of the largest scale that it has seen (at
@@ -250,6 +266,80 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, const PagedChunk& c
             pack2h<DT>(f[6], f[7])};
 }
 
+// One row by one wave on the vector ALUs, over its visible positions in [p0, p1): for tiles where
+// V holds NaN or infinities that some rows do not see (in a matrix product 0 * NaN is NaN).  64
+// positions at a time, one per lane; then the lanes hold columns lane, lane + 64, ...
+template <int DT, int CT, int HD>
+struct SlowRow {
+  static constexpr int N = (HD + 63) / 64;
+  float m, l, o[N];
+
+  static __device__ float value(const void* p, uint64_t i) {
+    if constexpr (CT == kE4M3) {
+      return __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<const uint8_t*>(p)[i], false)[0];
+    } else if constexpr (CT == kI8) {
+      return static_cast<float>(static_cast<const int8_t*>(p)[i]);
+    } else {
+      return u16_to_f32<CT>(static_cast<const uint16_t*>(p)[i]);
+    }
+  }
+  __device__ SlowRow(const AttnArgs& a, const PagedChunk& c, uint32_t b, uint32_t h, uint32_t row,
+                     uint32_t p0, uint32_t p1)
+      : m(-INFINITY), l(0.0f) {
+    const uint32_t lane = threadIdx.x & 63u, D = a.pool.head_dim;
+    const uint32_t end = min(p1, paged_visible(c, row / a.group));
+    const uint16_t* const q = a.q + (c.first + row / a.group) * a.q_stride +
+                              static_cast<uint64_t>(h * a.group + row % a.group) * D;
+    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+    for (uint32_t base = p0; base < end; base += 64) {
+      const uint32_t pos = base + lane;
+      const int32_t page = pos < end ? paged_page(a.seqs, b, pos) : -1;
+      const uint64_t at =
+          page < 0 ? 0 : pool_row(a.pool, a.seqs, page, h, paged_row(a.seqs, pos));
+      float s = -INFINITY, vs = 1.0f;
+      if (page >= 0) {
+        float dot = 0.0f;
+        for (uint32_t d = 0; d < D; ++d)
+          dot = __builtin_fmaf(u16_to_f32<DT>(q[d]), value(a.pool.k, at + d), dot);
+        s = dot * a.scale_log2;
+        if constexpr (cache_codes<CT>()) {
+          const uint64_t sc = pool_scale(a.pool, a.seqs, page, h, paged_row(a.seqs, pos));
+          s *= a.pool.k_scale[sc];
+          vs = a.pool.v_scale[sc];
+        }
+      }
+      const float mn = fmaxf(m, wave_max(s));
+      if (__builtin_amdgcn_ballot_w64(page >= 0) == 0) continue;
+      const float mu = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = m == -INFINITY ? 0.0f : exp2_fast(m - mu);
+      const float p = page < 0 ? 0.0f : exp2_fast(s - mu);
+      l = l * alpha + wave_sum(p);
+      m = mn;
+      for (int i = 0; i < N; ++i) o[i] *= alpha;
+      for (int x = 0; x < 64; ++x) {
+        const int32_t px = __builtin_amdgcn_readlane(page, x);
+        if (px < 0) continue;
+        const float w = __shfl(p * vs, x);
+        const uint64_t ax = read_lane64(at, x);
+        for (int i = 0; i < N; ++i) {
+          const uint32_t d = lane + 64 * i;
+          if (d < D) o[i] = __builtin_fmaf(w, value(a.pool.v, ax + d), o[i]);
+        }
+      }
+    }
+  }
+  __device__ void keep(float* p) const {
+    for (int i = 0; i < N; ++i) p[(threadIdx.x & 63u) + 64 * i] = o[i];
+  }
+  __device__ void write(uint16_t* p, uint32_t D) const {
+    for (int i = 0; i < N; ++i) {
+      const uint32_t d = (threadIdx.x & 63u) + 64 * i;
+      if (d < D)
+        p[d] = static_cast<uint16_t>(pack2h<DT>(l == 0.0f ? 0.0f : o[i] / l, 0.0f));
+    }
+  }
+};
+
 template <int DT, int CT, int HD, int MT>
 struct RowsTile {
   static constexpr bool kCodes = cache_codes<CT>();
@@ -383,37 +473,6 @@ struct RowsTile {
     }
   }
 
-  // The same for one tile on the vector ALUs, each row over the first `see` positions.  (Rare, so
-  // it is kept small: what it needs in registers is taken from all that comes before.)
-  static __device__ __forceinline__ void pv_seen(const char* lds, u32x4 pf, uint32_t see,
-                                                 f32x4 (&acc)[NC]) {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll 1
-      for (int gk = 0; gk < 4; ++gk) {
-        const uint32_t w = __shfl(pf[0], l16 + 16 * gk);
-        const float pk = u16_to_f32<DT>(static_cast<uint16_t>(w >> (16 * (i & 1))));
-        const uint32_t r = 16 * (i >> 2) + 4 * gk + (i & 3);
-        if (r < see) {
-#pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            uint32_t dg = 4 * g;
-            asm volatile("" : "+v"(dg) : : "memory");
-            const uint32_t d = 16 * c + dg;
-            const u32x2 x = *reinterpret_cast<const u32x2*>(lds + vaddr(r, d >> 3) + 2 * (d & 7));
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[c][j] = __builtin_fmaf(
-                  pk, u16_to_f32<DT>(static_cast<uint16_t>(x[j >> 1] >> (16 * (j & 1)))),
-                  acc[c][j]);
-          }
-        }
-      }
-      if (i & 1) pf = u32x4{pf[1], pf[2], pf[3], pf[0]};
-    }
-  }
-
   // Blocks [k0, k1) of tile `tile` of (b, h): the wave's share, then the workgroup's sum.
   // part: where the sums go, or null: O.
   static __device__ __forceinline__ void run(const AttnArgs& a, const PagedChunk& c, uint32_t b,
@@ -463,6 +522,7 @@ struct RowsTile {
       y.ev[i] = kExps ? kLeastExp : 0.0f;
     }
     char* const vlds = arena + wave * WB;
+    bool odd = false;   // NaN or infinities in V near the rows' ends
     if constexpr (MT > 1) __syncthreads();   // (Q of a pair of tiles leaves no registers for V)
 
     for (; base < end; base += rows::UNIT) {
@@ -489,11 +549,9 @@ struct RowsTile {
       }
       const bool there[2] = {st.page[0] >= 0, st.page[1] >= 0};
       const bool hides = base + 32 > vis_min || !there[0] || !there[1];   // uniform
-      bool odd = false;
       if (hides) {
 #pragma unroll
-        for (int i = 0; i < VL; ++i)
-          odd |= any_nonfinite<CT>(st.v[i]);
+        for (int i = 0; i < VL; ++i) odd |= any_nonfinite<CT>(st.v[i]);
       }
       float vs[8];
       if constexpr (kCodes) {
@@ -572,19 +630,15 @@ struct RowsTile {
         pf[i] = u32x4{pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
                       pack2h<DT>(p[6], p[7])};
       }
-      if (__builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max) {
-        // NaN or infinities among values that some rows do not see (0 * NaN is NaN)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-          pv_seen(vlds, pf[i], vis[i] > base ? vis[i] - base : 0u, y.acc[i]);
-      } else {
-        pv(vlds, pf, y);
-      }
+      pv(vlds, pf, y);
     }
 
     // the four waves' sums
     __shared__ float sm[4][TR], sl[4][TR];
+    __shared__ uint32_t odds[4];
     lds_order();
+    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max;
+    if (lane == 0) odds[wave] = any_odd;
     float* wo = reinterpret_cast<float*>(vlds);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -601,6 +655,23 @@ struct RowsTile {
       }
     }
     __syncthreads();
+    if ((odds[0] | odds[1] | odds[2] | odds[3]) != 0) {   // the whole workgroup
+      for (uint32_t r = wave; r < TR && r0 + r < nrows; r += 4) {
+        SlowRow<DT, CT, HD> x(a, c, b, h, r0 + r, k0 * rows::UNIT, k1 * rows::UNIT);
+        if (part) {
+          x.keep(part + r * HD);
+          if (lane == 0) {
+            part[TR * HD + r] = x.m;
+            part[TR * HD + TR + r] = x.l;
+          }
+        } else {
+          const uint64_t tok = c.first + (r0 + r) / G;
+          x.write(a.o + (tok * a.nh + h * G + (r0 + r) % G) * D, D);
+        }
+      }
+      __syncthreads();
+      return;
+    }
     constexpr int CPR = HD / 8;   // 8-value pieces of a row
     for (int x = t; x < TR * CPR; x += rows::NT) {
       const int r = x / CPR, c8 = 8 * (x % CPR);
@@ -747,8 +818,9 @@ __device__ __forceinline__ void rows_merge(const AttnArgs& a, uint32_t w) {
 namespace chunk {
 constexpr int NT = 512;
 constexpr int TR = 256;
-constexpr int KB = 64;           // positions of a block
-constexpr uint32_t kLeast = 8;   // blocks of a part, at least
+constexpr int KB = 64;            // positions of a block
+constexpr uint32_t RING = 2;      // blocks in LDS
+constexpr uint32_t kLeast = 512 / KB;   // blocks of a part, at least
 __host__ __device__ constexpr int rec(int hd) { return hd + 4; }   // O, then l, m
 
 // Tiles of a sequence, and the blocks of each part of one whose last row sees `vis` positions.
@@ -794,11 +866,11 @@ struct ChunkTile {
   static constexpr int NDS = HD / 16, NDT = HD / 32;
 
   struct Lds {
-    char kv[2][2 * KBYTES];
-    float ks[2][chunk::KB], vs[2][chunk::KB];   // 0 where nothing is held
-    float big[2];                               // scale_exp of the largest of vs
-    uint32_t there[2][4];                       // the pages of the block's four groups exist
-    uint32_t odd[2];                            // the block with NaN or infinities in V
+    char kv[chunk::RING][2 * KBYTES];
+    float ks[chunk::RING][chunk::KB], vs[chunk::RING][chunk::KB];   // 0 where nothing is held
+    float big[chunk::RING];          // scale_exp of the largest of vs
+    uint32_t there[chunk::RING][chunk::KB / 16];   // the pages of its groups of 16 exist
+    uint32_t odd;                    // NaN or infinities among V that some rows do not see
   };
   struct Stage {
     u32x4 k[XPT], v[XPT];
@@ -899,7 +971,7 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
   float m = -INFINITY, l = 0.0f, ev = T::kExps ? kLeastExp : 0.0f;
-  if (t < 2) sh.odd[t] = 0xffffffffu;
+  if (t == 0) sh.odd = 0;
 
   // this thread's pieces of a block: rows xr, 16-byte pieces xc.  A wave's rows, from wr on, lie
   // in one group of 16, so in one page.
@@ -914,15 +986,17 @@ attn_paged_chunk(AttnArgs a) {
   }
   const uint32_t rb = D * T::ESZ;
   typename T::Stage st;
-  int32_t id[XPT], id_s = -1;       // pages of the next block to be loaded
+  int32_t id[XPT], id_s = -1;       // pages of the next block to be loaded (id: unchecked)
   bool ok[XPT];                     // the stage's pages exist
   auto pages = [&](uint32_t j) {
     const uint32_t base = j * KB;
 #pragma unroll
     for (int i = 0; i < XPT; ++i)
-      id[i] = base + wr[i] < reach ? wave_page(a.seqs, b, base + wr[i]) : -1;
+      id[i] = wave_entry(a.seqs, b, base + wr[i], reach);
     if constexpr (T::kCodes)
-      id_s = t < 2 * KB && base + (t & 63) < reach ? paged_page(a.seqs, b, base + (t & 63)) : -1;
+      id_s = t < 2 * KB && base + (t & (KB - 1)) < reach
+                 ? paged_page(a.seqs, b, base + (t & (KB - 1)))
+                 : -1;
   };
   // Rows of missing pages and from `reach` on come as zeros, scales too.
   auto load = [&](uint32_t j) {
@@ -930,22 +1004,24 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < XPT; ++i) {
       const uint32_t pos = base + wr[i];
-      const uint32_t n = id[i] >= 0 && pos < reach ? min(64u / T::CPR, reach - pos) : 0u;
-      const uint64_t at = pool_row(a.pool, a.seqs, max(id[i], 0), h, paged_row(a.seqs, pos)) * T::ESZ;
+      const int32_t page = paged_checked(a.seqs, id[i]);
+      const uint32_t n = page >= 0 && pos < reach ? min(64u / T::CPR, reach - pos) : 0u;
+      const uint64_t at = pool_row(a.pool, a.seqs, max(page, 0), h, paged_row(a.seqs, pos)) * T::ESZ;
       const uint32_t off = 16 * xc[i] < rb ? (xr[i] - wr[i]) * rb + 16 * xc[i] : kPast;
       st.k[i] = load_within<false>(static_cast<const char*>(a.pool.k) + at, n * rb, off);
       st.v[i] = load_within<false>(static_cast<const char*>(a.pool.v) + at, n * rb, off);
-      ok[i] = id[i] >= 0;
+      ok[i] = page >= 0 || pos >= reach;   // (past reach nothing is seen anyway)
     }
     if constexpr (T::kCodes) {
       st.scale = 0.0f;
       if (id_s >= 0)
         st.scale = (t < KB ? a.pool.k_scale : a.pool.v_scale)[pool_scale(
-            a.pool, a.seqs, id_s, h, paged_row(a.seqs, base + (t & 63)))];
+            a.pool, a.seqs, id_s, h, paged_row(a.seqs, base + (t & (KB - 1))))];
     }
   };
+  auto slot = [&](uint32_t j) { return j % RING; };
   auto store = [&](uint32_t j) {   // what load(j) brought
-    char* const kl = sh.kv[j & 1];
+    char* const kl = sh.kv[slot(j)];
     char* const vl = kl + T::KBYTES;
     bool odd = false;
 #pragma unroll
@@ -966,209 +1042,212 @@ attn_paged_chunk(AttnArgs a) {
         *reinterpret_cast<u32x4*>(kl + T::kaddr(r, cc)) = k;
         *reinterpret_cast<u32x4*>(vl + T::vaddr(r, cc)) = v;
       }
-      if (cc == 0 && (r & 15) == 0) sh.there[j & 1][r >> 4] = ok[i];
+      if (cc == 0 && (r & 15) == 0) sh.there[slot(j)][r >> 4] = ok[i];
     }
     if constexpr (T::kCodes) {
-      if (t < 2 * KB) (t < KB ? sh.ks : sh.vs)[j & 1][t & 63] = st.scale;
+      if (t < 2 * KB) (t < KB ? sh.ks : sh.vs)[slot(j)][t & (KB - 1)] = st.scale;
       if constexpr (T::kExps) {
         if (wave == 1) {   // (its lanes hold all of vs)
+          static_assert(KB == 64, "vs in one wave");
           const float most = wave_max(st.scale);
-          if (lane == 0) sh.big[j & 1] = scale_exp(most);
+          if (lane == 0) sh.big[slot(j)] = scale_exp(most);
         }
       }
     }
-    if (odd && (j + 1) * KB > tile_min) sh.odd[j & 1] = j;   // (any of them: one value)
+    if (odd && (j + 1) * KB > tile_min) sh.odd = 1;   // (from any thread: one value)
   };
 
   const uint32_t vlane = T::vaddr(4 * (lane >> 5) + ((lane & 15) >> 2),
                                   (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) >> 3) +
                          2 * (4 * (lane & 3) & 7);
   const uint32_t klane = 128u * l32;
-  auto compute = [&](uint32_t j) {
-    const uint32_t base = j * KB;
-    if (base >= vis_max) return;   // uniform: nothing that the wave's rows see
-    const char* const kl = sh.kv[j & 1];
+  constexpr int NKT = KB / 32, NSP = KB / 16;
+  f32x16 s[NKT];        // a block's scores
+  u32x4 pf[NSP];        // its probabilities, 16 positions a step
+  // Products of block j: its scores (Q), or its probabilities with its V.  Fragments are read
+  // AHEAD products early, and the order is kept as written: left to itself the compiler reads so
+  // far ahead that registers spill.
+  auto products = [&](uint32_t j, auto q_) {
+    constexpr bool Q = decltype(q_)::value;
+    constexpr int N = Q ? NKT * T::NDS : NSP * T::NDT, AHEAD = 5;
+    const char* const kl = sh.kv[slot(j)];
     const char* const vl = kl + T::KBYTES;
-    f32x16 s[2];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
-#pragma unroll
-    for (int ds = 0; ds < T::NDS; ++ds)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(
-            kl + (ds >> 2) * (KB * 128) + kt * 4096 + klane +
-            16 * ((2 * (ds & 3) + g) ^ T::kswz(l32)));
-        s[kt] = mfma32x32x16<DT>(kf, qf[ds], s[kt]);
+    u32x4 frag[AHEAD + 1];
+    auto read = [&](int i) {
+      u32x4& f = frag[i % (AHEAD + 1)];
+      if constexpr (Q) {
+        const int ds = i / NKT, kt = i % NKT;
+        f = *reinterpret_cast<const u32x4*>(kl + (ds >> 2) * (KB * 128) + kt * 4096 + klane +
+                                            16 * ((2 * (ds & 3) + g) ^ T::kswz(l32)));
+      } else {
+        // columns 32 dt on: chunk bits 2 and up, which the swizzle's bit 2 meets by XOR
+        const int sp = i / T::NDT, dt = i % T::NDT;
+        const uint32_t va = vlane ^ (dt << 6);
+        const u32x2 lo = lds::read_tr16(vl + va + 16 * T::RB * sp);
+        const u32x2 hi = lds::read_tr16(vl + va + 16 * T::RB * sp + 8 * T::RB);
+        f = u32x4{lo[0], lo[1], hi[0], hi[1]};
       }
-    // lane (row l32, g): accumulator r of half kt is position base + 32 kt + 8 (r / 4) + 4 g + r % 4
+    };
+    if constexpr (Q) {
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD && i < N; ++i) read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + AHEAD < N) read(i + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x4 f = frag[i % (AHEAD + 1)];
+      if constexpr (Q) s[i % NKT] = mfma32x32x16<DT>(f, qf[i / NKT], s[i % NKT]);
+      else acc[i % T::NDT] = mfma32x32x16<DT>(f, pf[i / T::NDT], acc[i % T::NDT]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto softmax = [&](uint32_t j) {
+    const uint32_t base = j * KB, at_ring = slot(j);
+    // lane (row l32, g): accumulator r of s[kt] is position base + 32 kt + 8 (r / 4) + 4 g + r % 4
     if constexpr (T::kCodes) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int q = 0; q < 4 * NKT; ++q) {
+        const f32x4 ks = *reinterpret_cast<const f32x4*>(&sh.ks[at_ring][8 * q + 4 * g]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 ks = *reinterpret_cast<const f32x4*>(&sh.ks[j & 1][32 * kt + 8 * q + 4 * g]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[kt][4 * q + i] *= ks[i];
-        }
+        for (int i = 0; i < 4; ++i) s[q >> 2][4 * (q & 3) + i] *= ks[i];
+      }
     }
     uint32_t there = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) there |= sh.there[j & 1][i] << i;
+    for (int i = 0; i < NSP; ++i) there |= sh.there[at_ring][i] << i;
     there = __builtin_amdgcn_readfirstlane(there);
-    const bool hides = base + KB > vis_min || there != 15;
+    const bool hides = base + KB > vis_min || there != (1u << NSP) - 1;
     const int lim = static_cast<int>(vis) - static_cast<int>(base) - 4 * g;
     if (hides) {
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
-          const int lim_g = there >> (at >> 4) & 1 ? lim : -64;   // (uniform)
-          s[kt][i] = at < lim_g ? s[kt][i] : -INFINITY;
-        }
+      for (int i = 0; i < 16 * NKT; ++i) {
+        const int at = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+        const int lim_g = there >> (at >> 4) & 1 ? lim : -64;   // (uniform)
+        s[i >> 4][i & 15] = at < lim_g ? s[i >> 4][i & 15] : -INFINITY;
+      }
     }
-    float mx[4];
+    float mx[NSP];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < NSP; ++q) {
       mx[q] = s[q >> 1][8 * (q & 1)];
 #pragma unroll
       for (int i = 1; i < 8; ++i) mx[q] = fmaxf(mx[q], s[q >> 1][8 * (q & 1) + i]);
     }
-    const float top = pair_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * a.scale_log2;
+#pragma unroll
+    for (int q = 1; q < NSP; ++q) mx[0] = fmaxf(mx[0], mx[q]);
+    const float top = pair_max(mx[0]) * a.scale_log2;
     float big = kLeastExp;
     if constexpr (T::kExps) {
       if (hides) {
         float most = 0.0f;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * kt + 8 * (i >> 2) + (i & 3);
-            most = fmaxf(most, at < lim ? sh.vs[j & 1][at + 4 * g] : 0.0f);
-          }
+        for (int i = 0; i < 16 * NKT; ++i) {
+          const int at = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+          most = fmaxf(most, at < lim ? sh.vs[at_ring][at + 4 * g] : 0.0f);
+        }
         big = scale_exp(pair_max(most));
       } else {
-        big = sh.big[j & 1];
+        big = sh.big[at_ring];
       }
     }
-    float alpha = 1.0f;
-    bool moved = false;
     if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || (T::kExps && big > ev)) != 0) {
       const float old = m + ev;
       m = fmaxf(m, top);
       ev = T::kExps ? fmaxf(ev, big) : 0.0f;
-      alpha = m == -INFINITY ? 1.0f : exp2_fast(old - (m + ev));
+      const float alpha = m == -INFINITY ? 1.0f : exp2_fast(old - (m + ev));
       l *= alpha;
-      moved = true;
-    }
-    const float mu = m == -INFINITY ? 0.0f : m + ev;
-    float l0 = 0.0f, l1 = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kt][i] = exp2_fast(__builtin_fmaf(s[kt][i], a.scale_log2, -mu));
-        (i & 1 ? l1 : l0) += s[kt][i];
-      }
-    l += l0 + l1;
-    if (moved) {
 #pragma unroll
       for (int i = 0; i < T::NDT; ++i)
 #pragma unroll
         for (int x = 0; x < 16; ++x) acc[i][x] *= alpha;
     }
-    // the probabilities of PV step sp, by their positions' scales
-    auto weigh = [&](int sp) {
+    const float mu = m == -INFINITY ? 0.0f : m + ev;
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int sp = 0; sp < NSP; ++sp) {   // the product with V takes 16 positions a step
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = exp2_fast(__builtin_fmaf(s[sp >> 1][8 * (sp & 1) + i], a.scale_log2, -mu));
+        (i & 1 ? l1 : l0) += p[i];
+      }
       if constexpr (T::kCodes) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int at = 16 * sp + 8 * q;
-          const f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[j & 1][at + 4 * g]);
+          const f32x4 vs = *reinterpret_cast<const f32x4*>(&sh.vs[at_ring][at + 4 * g]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int x = 8 * (sp & 1) + 4 * q + i;
-            s[sp >> 1][x] *= vs[i];
-            if (hides) s[sp >> 1][x] = at + i < lim ? s[sp >> 1][x] : 0.0f;   // (may be NaN)
+            p[4 * q + i] *= vs[i];
+            if (hides) p[4 * q + i] = at + i < lim ? p[4 * q + i] : 0.0f;   // (vs may be NaN)
           }
         }
       }
-    };
-    if (hides && __builtin_amdgcn_readfirstlane(sh.odd[j & 1]) == j && vis_min < reach) {
-#pragma unroll
-      for (int sp = 0; sp < 4; ++sp) weigh(sp);
-      // NaN or infinities among values that some rows do not see (0 * NaN is NaN): this block on
-      // the vector ALUs, each row over what it sees
-#pragma unroll 1
-      for (int i = 0; i < 32; ++i) {
-#pragma unroll 1
-        for (int gk = 0; gk < 2; ++gk) {
-          const float pk = __shfl(s[0][0], l32 + 32 * gk);
-          const uint32_t r = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * gk + (i & 3);
-          if (base + r < vis) {
-#pragma unroll
-            for (int x = 0; x < 4 * T::NDT; ++x) {
-              uint32_t dg = 4 * g;
-              asm volatile("" : "+v"(dg) : : "memory");   // (few registers, as for the rows)
-              const uint32_t d = 8 * x + dg;
-              const u32x2 v =
-                  *reinterpret_cast<const u32x2*>(vl + T::vaddr(r, d >> 3) + 2 * (d & 7));
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                acc[x >> 2][4 * (x & 3) + y] = __builtin_fmaf(
-                    pk, u16_to_f32<DT>(static_cast<uint16_t>(v[y >> 1] >> (16 * (y & 1)))),
-                    acc[x >> 2][4 * (x & 3) + y]);
-            }
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < 31; ++x) s[x >> 4][x & 15] = s[(x + 1) >> 4][(x + 1) & 15];
-      }
-      return;
+      pf[sp] = u32x4{pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
+                     pack2h<DT>(p[6], p[7])};
     }
-#pragma unroll
-    for (int sp = 0; sp < 4; ++sp) {
-      const int o = 8 * (sp & 1);
-      weigh(sp);
-      const f32x16& p = s[sp >> 1];
-      const u32x4 pf = {pack2h<DT>(p[o], p[o + 1]), pack2h<DT>(p[o + 2], p[o + 3]),
-                        pack2h<DT>(p[o + 4], p[o + 5]), pack2h<DT>(p[o + 6], p[o + 7])};
-#pragma unroll
-      for (int dt = 0; dt < T::NDT; ++dt) {
-        // columns 32 dt on: chunk bits 2 and up, which the swizzle's bit 2 meets by XOR
-        const uint32_t va = vlane ^ (dt << 6);
-        const u32x2 lo = lds::read_tr16(vl + va + 16 * T::RB * sp);
-        const u32x2 hi = lds::read_tr16(vl + va + 16 * T::RB * sp + 8 * T::RB);
-        acc[dt] = mfma32x32x16<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, acc[dt]);
-      }
-    }
+    l += l0 + l1;
+  };
+  // Block j, loaded a block ago, into LDS, and the next one on its way.  (Past the last block
+  // these are zeros, and nothing is read.)
+  auto bring = [&](uint32_t j) {
+    store(j);
+    load(j + 1);
+    pages(j + 2);
+  };
+  auto turn = [&] {   // this wave's LDS writes are done, then everyone's
+    lds::wait_lgkm0();
+    lds::bar();
   };
 
   if (j0 < j1) {
+    // Every wave takes part in bringing every block; those from jw on have nothing that its rows
+    // see.  (The accumulators change in one straight line of code: with branches around the
+    // products the compiler copies them back and forth.)
+    const uint32_t jw = max(j0, min(j1, (vis_max + KB - 1) / KB));
     pages(j0);
     load(j0);
-    if (j0 + 1 < j1) pages(j0 + 1);
-    __syncthreads();   // (sh.odd)
-    store(j0);
-    if (j0 + 1 < j1) {
-      load(j0 + 1);
-      }
-    if (j0 + 2 < j1) pages(j0 + 2);
-    for (uint32_t j = j0; j < j1; ++j) {
-      // block j is whole in LDS, and every wave is done with block j - 1, whose half block
-      // j + 1 takes
-      __syncthreads();
-      if (j + 1 < j1) store(j + 1);
-      if (j + 2 < j1) {
-        load(j + 2);
-          }
-      if (j + 3 < j1) pages(j + 3);
-      compute(j);
+    pages(j0 + 1);
+    turn();   // (sh.odd)
+    bring(j0);
+    turn();
+    for (uint32_t j = j0; j < jw; ++j) {
+      bring(j + 1);   // its place in the ring was last read before the last turn
+      products(j, std::true_type{});
+      softmax(j);
+      products(j, std::false_type{});
+      turn();
+    }
+    for (uint32_t j = jw; j < j1; ++j) {
+      bring(j + 1);
+      turn();
     }
   }
   if (!live_wave) return;
+  auto record = [&](uint64_t at) {
+    return a.chunk_ws + (static_cast<uint64_t>(part) * a.seqs.total_q * a.nh + at) * rec(HD);
+  };
+  if (j0 < j1 && __builtin_amdgcn_readfirstlane(sh.odd) != 0) {   // (set before the last turn)
+    for (uint32_t r = wr0; r < min(nrows, wr0 + 32); ++r) {
+      SlowRow<DT, CT, HD> y(a, c, b, h, r, j0 * KB, j1 * KB);
+      const uint64_t at = (c.first + r / G) * static_cast<uint64_t>(a.nh) + h * G + r % G;
+      if (whole) {
+        y.write(a.o + at * D, D);
+      } else {
+        y.keep(record(at));
+        if (lane == 0) {
+          record(at)[HD] = y.l;
+          record(at)[HD + 1] = y.m;
+        }
+      }
+    }
+    return;
+  }
   l = pair_sum(l);
   if (!live_row) return;
   const uint64_t at = (c.first + qi) * static_cast<uint64_t>(a.nh) + hq;
@@ -1187,18 +1266,16 @@ attn_paged_chunk(AttnArgs a) {
               u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
       }
   } else {
-    float* const rec_ =
-        a.chunk_ws +
-        (static_cast<uint64_t>(part) * a.seqs.total_q * a.nh + at) * rec(HD);
+    float* const out = record(at);
 #pragma unroll
     for (int i = 0; i < T::NDT; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(rec_ + 32 * i + 8 * q + 4 * g) =
+        *reinterpret_cast<f32x4*>(out + 32 * i + 8 * q + 4 * g) =
             f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
     if (g == 0) {
-      rec_[HD] = l;
-      rec_[HD + 1] = m + ev;
+      out[HD] = l;
+      out[HD + 1] = m + ev;
     }
   }
 }
