@@ -744,6 +744,8 @@ attn_paged_rows(AttnArgs a) {
   }
 }
 
+constexpr int merge_nt = 512;
+
 // Merge the parts of a tile that several runs share.  Workgroup w looks after the tile in which
 // run w + 1 begins, if run w holds that tile's first unit: parts 2 w + 1, then 2 (w + 1), ...
 // One wave per row, HD / 8 lanes per part of it.
@@ -771,7 +773,7 @@ __device__ __forceinline__ void rows_merge(const AttnArgs& a, uint32_t w) {
   const int lane = threadIdx.x & 63;
   constexpr int CPR = HD / 8, PG = 64 / CPR;   // parts that a wave reads at once
   const int c8 = 8 * (lane % CPR), pg = lane / CPR;
-  for (uint32_t r = threadIdx.x >> 6; r < TR && r0 + r < nrows; r += 4) {
+  for (uint32_t r = threadIdx.x >> 6; r < TR && r0 + r < nrows; r += merge_nt / 64) {
     float M = -INFINITY, o[8], ls = 0.0f;
     for (uint32_t i = lane; i < np; i += 64) M = fmaxf(M, rec(i)[TR * HD + r]);
 #pragma unroll
@@ -904,34 +906,53 @@ attn_paged_chunk(AttnArgs a) {
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t nkv = a.pool.nkv, D = a.pool.head_dim, G = a.group;
 
-  // item: heads fastest (workgroup w runs on XCD w % 8, so a head's tiles share an L2 where
-  // there are eight), then parts, then tiles from the last (longest) on, then sequences
+  // Item: heads fastest (workgroup w runs on XCD w % 8, so a head's tiles share an L2 where there
+  // are eight), then parts, then the sequences that have a tile t, t from the largest down: about
+  // the longest first, which leaves the shortest for the end.  (Five prompts of up to 2000 tokens:
+  // the longest CU had 47 blocks' work sequence by sequence, 36 so, of 30 on average.)
   const uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.x % nkv);
   const uint32_t part = __builtin_amdgcn_readfirstlane(blockIdx.x / nkv % a.parts);
   uint32_t left = blockIdx.x / nkv / a.parts, b = 0;
   {
-    bool found = false;
-    for (uint32_t b0 = 0; b0 < a.seqs.batch && !found; b0 += 64) {
-      const uint32_t n =
-          b0 + lane < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, b0 + lane)) : 0u;
-      uint32_t inc = n;
+    const uint32_t own =
+        static_cast<uint32_t>(lane) < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, lane)) : 0u;
+    auto tiles_of = [&](uint32_t b0) {   // of sequence b0 + lane
+      if (b0 == 0) return own;
+      return b0 + lane < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, b0 + lane)) : 0u;
+    };
+    auto from = [&](uint32_t t) {   // tiles t and later of all sequences
+      uint32_t n = 0;
+      for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
+        const uint32_t x = tiles_of(b0);
+        n += x > t ? x - t : 0u;
+      }
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t x = __shfl_up(inc, d);
-        if (lane >= d) inc += x;
-      }
-      const uint64_t in = __builtin_amdgcn_ballot_w64(left < inc);
-      if (in != 0) {
-        const int l = __builtin_ctzll(in);
-        b = b0 + l;
-        // tiles of this sequence from the last
-        left = __builtin_amdgcn_readlane(static_cast<int>(inc), l) - 1 - left;
-        found = true;
-      } else {
-        left -= __builtin_amdgcn_readlane(static_cast<int>(inc), 63);
-      }
+      for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
+      return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(n));
+    };
+    if (left >= from(0)) return;
+    uint32_t lo = 0, hi = 1;   // from(lo) > left >= from(hi)
+    while (from(hi) > left) {
+      lo = hi;
+      hi *= 2;
     }
-    if (!found) return;
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      if (from(mid) > left) lo = mid;
+      else hi = mid;
+    }
+    left -= from(lo + 1);
+    for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
+      uint64_t in = __builtin_amdgcn_ballot_w64(tiles_of(b0) > lo);
+      const uint32_t n = __builtin_popcountll(in);
+      if (left < n) {
+        for (; left > 0; --left) in &= in - 1;
+        b = b0 + __builtin_ctzll(in);
+        break;
+      }
+      left -= n;
+    }
+    left = lo;
   }
   const uint32_t tile = __builtin_amdgcn_readfirstlane(left);
   const PagedChunk c = paged_chunk(a.seqs, b);
@@ -1280,55 +1301,72 @@ attn_paged_chunk(AttnArgs a) {
   }
 }
 
-// Merge a chunk tile's parts: one workgroup per token, HD / 4 lanes per row.
+// Merge a chunk tile's parts: rows of one token, HD / 4 lanes per row, four parts' loads at once.
 template <int DT, int HD>
-__device__ __forceinline__ void chunk_merge(const AttnArgs& a, uint32_t token) {
+__device__ __forceinline__ void chunk_merge(const AttnArgs& a, uint32_t item) {
   using namespace chunk;
-  constexpr int LPR = HD / 4, RPB = 256 / LPR;
-  const uint32_t lane = threadIdx.x & 63u;
+  constexpr uint32_t LPR = HD / 4, RPB = merge_nt / LPR;
+  const uint32_t groups = (a.nh + RPB - 1) / RPB;
+  const uint32_t lane = threadIdx.x & 63u, token = item / groups;
+  const uint32_t hq = item % groups * RPB + threadIdx.x / LPR;
   uint32_t le = 0;
   for (uint32_t j0 = 0; j0 < a.seqs.batch; j0 += 64) {
     const uint32_t j = j0 + lane;
     le += __builtin_popcountll(__builtin_amdgcn_ballot_w64(
         j < a.seqs.batch && paged_clamp(a.seqs.q_start[j], a.seqs.total_q) <= token));
   }
-  if (le == 0) return;
+  if (le == 0 || hq >= a.nh) return;
   const PagedChunk c = paged_chunk(a.seqs, le - 1);
   if (token < c.first || token - c.first >= c.n || c.n * a.group <= a.split_rows) return;
   const int d = 4 * (threadIdx.x % LPR);
-  for (uint32_t hq = threadIdx.x / LPR; hq < a.nh; hq += RPB) {
-    const uint32_t row = (token - c.first) * a.group + hq % a.group;
-    const uint32_t reach = tile_reach(a, c, row / TR);
-    const uint32_t per = part_blocks(reach, a.parts), nb = (reach + KB - 1) / KB;
-    if (per >= nb) continue;
-    const uint32_t np = (nb + per - 1) / per;
-    const uint64_t step = static_cast<uint64_t>(a.seqs.total_q) * a.nh * rec(HD);
-    const float* r = a.chunk_ws + (static_cast<uint64_t>(token) * a.nh + hq) * rec(HD);
-    float M = -INFINITY;
-    for (uint32_t p = 0; p < np; ++p) M = fmaxf(M, r[p * step + HD + 1]);
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t p = 0; p < np; ++p) {
-      const float lp = r[p * step + HD], mp = r[p * step + HD + 1];
-      if (lp == 0.0f) continue;   // a part that the row sees nothing of
-      const float w = mp == -INFINITY ? 0.0f : exp2_fast(mp - M);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(r + p * step + d);
-      l = __builtin_fmaf(w, lp, l);
+  const uint32_t row = (token - c.first) * a.group + hq % a.group;
+  const uint32_t reach = tile_reach(a, c, row / TR);
+  const uint32_t per = part_blocks(reach, a.parts), nb = (reach + KB - 1) / KB;
+  if (per >= nb) return;
+  const uint32_t np = (nb + per - 1) / per;
+  const uint64_t step = static_cast<uint64_t>(a.seqs.total_q) * a.nh * rec(HD);
+  const float* r = a.chunk_ws + (static_cast<uint64_t>(token) * a.nh + hq) * rec(HD);
+  float M = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t p0 = 0; p0 < np; p0 += 4) {
+    f32x4 x[4];
+    float lp[4], mp[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(w, x[i], o[i]);
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float* q = r + min(p0 + i, np - 1) * step;
+      x[i] = *reinterpret_cast<const f32x4*>(q + d);
+      lp[i] = p0 + i < np ? q[HD] : 0.0f;
+      mp[i] = q[HD + 1];
     }
-    if (d < static_cast<int>(a.pool.head_dim)) {
-      float f[4];
+    float top = M;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = l == 0.0f ? 0.0f : o[i] / l;
-      *reinterpret_cast<u32x2*>(a.o + (static_cast<uint64_t>(token) * a.nh + hq) * a.pool.head_dim +
-                                d) = u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
+    for (int i = 0; i < 4; ++i) top = lp[i] == 0.0f ? top : fmaxf(top, mp[i]);
+    const float keep = M == -INFINITY ? 0.0f : exp2_fast(M - top);
+    M = top;
+    l *= keep;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = M == -INFINITY ? o[j] : o[j] * keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (lp[i] == 0.0f) continue;   // a part that the row sees nothing of
+      const float w = mp[i] == -INFINITY ? 0.0f : exp2_fast(mp[i] - M);
+      l = __builtin_fmaf(w, lp[i], l);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(w, x[i][j], o[j]);
     }
+  }
+  if (d < static_cast<int>(a.pool.head_dim)) {
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = l == 0.0f ? 0.0f : o[i] / l;
+    *reinterpret_cast<u32x2*>(a.o + (static_cast<uint64_t>(token) * a.nh + hq) * a.pool.head_dim +
+                              d) = u32x2{pack2h<DT>(f[0], f[1]), pack2h<DT>(f[2], f[3])};
   }
 }
 
-// Both kernels' merges in one launch: `first` workgroups for the rows' runs, then one per token.
+// Both kernels' merges in one launch: `first` workgroups for the rows' runs, then those of the
+// chunks' tokens.
 template <int DT, int HD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(merge_nt)
 attn_paged_merge(AttnArgs a, uint32_t first) {
   if (blockIdx.x < first) {
     rows_merge<DT, HD>(a, blockIdx.x);

@@ -171,9 +171,11 @@ void attn_paged_go(const th::pgd::AttnArgs& a, const AttnPlan& p, hipStream_t s)
                          0, s, a);
   }
   const uint32_t first = p.rows_merge ? p.runs - 1 : 0;
-  const uint32_t tokens = p.items && p.parts > 1 ? a.seqs.total_q : 0;
-  if (first + tokens)   // below 2^31: total_q and a few runs
-    hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, HD>), dim3(first + tokens), dim3(256), 0, s,
+  constexpr uint32_t MNT = th::pgd::merge_nt, RPB = MNT / (HD / 4);   // (chunk_merge)
+  const uint32_t tokens =
+      p.items && p.parts > 1 ? a.seqs.total_q * ((a.nh + RPB - 1) / RPB) : 0;   // parts: some 10^4 rows
+  if (first + tokens)
+    hipLaunchKernelGGL((th::pgd::attn_paged_merge<DT, HD>), dim3(first + tokens), dim3(MNT), 0, s,
                        a, first);
 }
 
