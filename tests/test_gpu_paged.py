@@ -388,6 +388,18 @@ def test_many_sequences(dev, stream, batch):
     check_attention(dev, stream, pool, table, start, length, q, D.BF16, 4)
 
 
+@pytest.mark.parametrize("batch", [64, 65, 140])
+def test_many_chunks(dev, stream, batch):
+    """Chunks of several row tiles in as many sequences as one look at the lengths takes, and in
+    more; idle sequences between."""
+    rng = np.random.default_rng(batch)
+    length = rng.integers(0, 200, batch).tolist()
+    new = [0 if b % 9 == 4 else min(n, int(x))
+           for b, (n, x) in enumerate(zip(length, rng.integers(0, 200, batch)))]
+    pool, table, start, q = make(rng, D.E4M3, D.F16, 1, 4, 64, 16, length, new)
+    check_attention(dev, stream, pool, table, start, length, q, D.F16, 4)
+
+
 def test_long_step_is_the_same_twice(dev, stream):
     """One sequence over many runs: within the bound, the same bits each time, also on the
     stream's own scratch."""

@@ -82,6 +82,12 @@ def test_refusals_of_one_call():
     refused("stride", lambda: th.kv_cache_write(p, s, a, a, D.BF16, stride=132))
     refused("stride", lambda: th.kv_cache_write(p, s, a, a, D.F32, stride=130))
     refused("stride is too large", lambda: th.kv_cache_write(p, s, a, a, D.F32, stride=1 << 60))
+    many = structs(total_q=1 << 28)[1]
+    refused("grid too large", lambda: th.kv_cache_write(p, many, a, a, D.F32))
+    refused("grid too large", lambda: th.kv_cache_read(p, s, a, a, 0x7fffffff, D.F32))
+    refused("grid too large", lambda: th.attention_paged(a, p, structs(batch=1 << 28,
+                                                                       total_q=1 << 29)[1], a, 2,
+                                                         D.BF16))
     refused("null pointer", lambda: th.kv_cache_write(p, s, 0, a, D.BF16))
     refused("aligned", lambda: th.kv_cache_write(p, s, a, a + 2, D.BF16))
     refused("unknown dtype", lambda: th.kv_cache_read(p, s, a, a, 8, D.I8))
@@ -100,6 +106,8 @@ def test_refusals_of_one_call():
     refused("aligned", lambda: th.attention_paged(a, p, s, a + 8, 4, D.BF16))
     big, many = structs(total_q=1 << 30)
     refused("total_q * num_heads", lambda: th.attention_paged(a, big, many, a, 4, D.BF16))
+    assert th.attention_paged_workspace_size(p, s, 4) == 0   # 48 positions: nothing is split
+    p, s = structs(max_pages=30)
     room = th.attention_paged_workspace_size(p, s, 4)
     assert room > 0
     refused("workspace", lambda: th.attention_paged(a, p, s, a, 4, D.BF16, workspace=a,

@@ -907,28 +907,22 @@ attn_paged_chunk(AttnArgs a) {
   const uint32_t nkv = a.pool.nkv, D = a.pool.head_dim, G = a.group;
 
   // Item: heads fastest (workgroup w runs on XCD w % 8, so a head's tiles share an L2 where there
-  // are eight), then parts, then the sequences that have a tile t, t from the largest down: about
-  // the longest first, which leaves the shortest for the end.  (Five prompts of up to 2000 tokens:
-  // the longest CU had 47 blocks' work sequence by sequence, 36 so, of 30 on average.)
+  // are eight), then parts, then tiles.  Of up to 64 sequences, those that have a tile t, t from
+  // the largest down: about the longest first, which leaves the shortest for the end.  (Five
+  // prompts of up to 2000 tokens, 64-wide e4m3: 113 -> 103 us; the longest CU had 47 blocks' work
+  // sequence by sequence, 36 so, of 30 on average.)  Of more, whose items fill the CUs many times,
+  // sequence by sequence, each from its last tile on, in one pass over the lengths.
   const uint32_t h = __builtin_amdgcn_readfirstlane(blockIdx.x % nkv);
   const uint32_t part = __builtin_amdgcn_readfirstlane(blockIdx.x / nkv % a.parts);
   uint32_t left = blockIdx.x / nkv / a.parts, b = 0;
-  {
-    const uint32_t own =
-        static_cast<uint32_t>(lane) < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, lane)) : 0u;
-    auto tiles_of = [&](uint32_t b0) {   // of sequence b0 + lane
-      if (b0 == 0) return own;
-      return b0 + lane < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, b0 + lane)) : 0u;
-    };
+  if (a.seqs.batch <= 64) {
+    const uint32_t n = static_cast<uint32_t>(lane) < a.seqs.batch
+                           ? tiles(a, paged_chunk(a.seqs, lane)) : 0u;
     auto from = [&](uint32_t t) {   // tiles t and later of all sequences
-      uint32_t n = 0;
-      for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
-        const uint32_t x = tiles_of(b0);
-        n += x > t ? x - t : 0u;
-      }
+      uint32_t sum = n > t ? n - t : 0u;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-      return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(n));
+      for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+      return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(sum));
     };
     if (left >= from(0)) return;
     uint32_t lo = 0, hi = 1;   // from(lo) > left >= from(hi)
@@ -941,18 +935,32 @@ attn_paged_chunk(AttnArgs a) {
       if (from(mid) > left) lo = mid;
       else hi = mid;
     }
-    left -= from(lo + 1);
-    for (uint32_t b0 = 0; b0 < a.seqs.batch; b0 += 64) {
-      uint64_t in = __builtin_amdgcn_ballot_w64(tiles_of(b0) > lo);
-      const uint32_t n = __builtin_popcountll(in);
-      if (left < n) {
-        for (; left > 0; --left) in &= in - 1;
-        b = b0 + __builtin_ctzll(in);
-        break;
-      }
-      left -= n;
-    }
+    uint64_t in = __builtin_amdgcn_ballot_w64(n > lo);
+    for (left -= from(hi); left > 0; --left) in &= in - 1;
+    b = __builtin_ctzll(in);
     left = lo;
+  } else {
+    bool found = false;
+    for (uint32_t b0 = 0; b0 < a.seqs.batch && !found; b0 += 64) {
+      const uint32_t n =
+          b0 + lane < a.seqs.batch ? tiles(a, paged_chunk(a.seqs, b0 + lane)) : 0u;
+      uint32_t inc = n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t x = __shfl_up(inc, d);
+        if (lane >= d) inc += x;
+      }
+      const uint64_t in = __builtin_amdgcn_ballot_w64(left < inc);
+      if (in != 0) {
+        const int l = __builtin_ctzll(in);
+        b = b0 + l;
+        left = __builtin_amdgcn_readlane(static_cast<int>(inc), l) - 1 - left;
+        found = true;
+      } else {
+        left -= __builtin_amdgcn_readlane(static_cast<int>(inc), 63);
+      }
+    }
+    if (!found) return;
   }
   const uint32_t tile = __builtin_amdgcn_readfirstlane(left);
   const PagedChunk c = paged_chunk(a.seqs, b);

@@ -40,22 +40,34 @@ __device__ __forceinline__ uint64_t pool_scale(const PagedPool& p, const PagedSe
   return ((static_cast<uint64_t>(page) * p.nkv + head) << s.shift) + row;
 }
 
-// Eight values of a tensor of type DT from p, in f32, and back (one rounding).
+// Eight values of a tensor of type DT as they lie in memory; their values in f32, and back (one
+// rounding).
+template <int DT> struct Raw8 {
+  u32x4 w[DT == kF32 ? 2 : 1];
+};
 template <int DT>
-__device__ __forceinline__ void load8(const void* p, float (&f)[8]) {
-  if constexpr (DT == kF32) {
-    const u32x4 a = ldg128(p), b = ldg128(static_cast<const float*>(p) + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = __uint_as_float(a[i]);
-      f[4 + i] = __uint_as_float(b[i]);
-    }
-  } else {
-    unpack16<DT>(ldg128(p), f);
-  }
+__device__ __forceinline__ Raw8<DT> load8(const void* p) {
+  Raw8<DT> r;
+  r.w[0] = ldg128(p);
+  if constexpr (DT == kF32) r.w[1] = ldg128(static_cast<const float*>(p) + 4);
+  return r;
 }
 template <int DT>
+__device__ __forceinline__ void widen8(const Raw8<DT>& r, float (&f)[8]) {
+  if constexpr (DT == kF32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r.w[i / 4][i % 4]);
+  } else {
+    unpack16<DT>(r.w[0], f);
+  }
+}
+// (Past: around the caches.)
+template <int DT, bool Past>
 __device__ __forceinline__ void store8(void* p, const float (&f)[8]) {
+  auto put = [](u32x4 x, u32x4* to) {
+    if constexpr (Past) __builtin_nontemporal_store(x, to);
+    else *to = x;
+  };
   if constexpr (DT == kF32) {
     u32x4 a, b;
 #pragma unroll
@@ -63,10 +75,10 @@ __device__ __forceinline__ void store8(void* p, const float (&f)[8]) {
       a[i] = __float_as_uint(f[i]);
       b[i] = __float_as_uint(f[4 + i]);
     }
-    *static_cast<u32x4*>(p) = a;
-    *(static_cast<u32x4*>(p) + 1) = b;
+    put(a, static_cast<u32x4*>(p));
+    put(b, static_cast<u32x4*>(p) + 1);
   } else {
-    *static_cast<u32x4*>(p) = pack16<DT>(f);
+    put(pack16<DT>(f), static_cast<u32x4*>(p));
   }
 }
 
@@ -83,14 +95,16 @@ __device__ __forceinline__ u32x2 encode8(const float (&f)[8]) {
       w[i] = static_cast<uint32_t>(d);
     }
   } else {
+    // f + 3 * 2^22 has the integer nearest to f (ties to even) in its low bits: at most 127
+    // (1 + 2^-22), so in its low byte
+    uint32_t d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = __float_as_uint(f[i] + 12582912.0f);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint32_t d = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        d |= (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(f[4 * i + j]))) & 0xffu)
-             << (8 * j);
-      w[i] = d;
+      const uint32_t lo = __builtin_amdgcn_perm(d[4 * i + 1], d[4 * i], 0x0c0c0400u);
+      const uint32_t hi = __builtin_amdgcn_perm(d[4 * i + 3], d[4 * i + 2], 0x04000c0cu);
+      w[i] = lo | hi;
     }
   }
   return w;
@@ -127,6 +141,19 @@ kv_cache_write(PagedPool p, PagedSeqs s, const void* __restrict__ k, const void*
   const uint32_t token =
       __builtin_amdgcn_readfirstlane(blockIdx.x * 4u + (threadIdx.x >> 6));
   if (token >= s.total_q) return;
+  const uint32_t col = 8u * (lane % LG), rows = 2u * p.nkv;
+  Raw8<DT> x[U];
+  auto bring = [&](uint32_t r0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t r = r0 + u * RPW, h = r < p.nkv ? r : r - p.nkv;
+      x[u] = {};
+      if (r < rows && col < p.head_dim)
+        x[u] = load8<DT>(static_cast<const char*>(r < p.nkv ? k : v) +
+                         SZ * (token * stride + static_cast<uint64_t>(h) * p.head_dim + col));
+    }
+  };
+  bring(lane / LG);   // in flight while the sequence is looked up
   uint32_t le = 0;
   for (uint32_t j0 = 0; j0 < s.batch; j0 += 64) {
     const uint32_t j = j0 + lane;
@@ -142,46 +169,42 @@ kv_cache_write(PagedPool p, PagedSeqs s, const void* __restrict__ k, const void*
   const int32_t page = paged_page(s, b, static_cast<uint32_t>(pos));
   if (page < 0) return;
   const uint32_t row = paged_row(s, static_cast<uint32_t>(pos));
-  const uint32_t col = 8u * (lane % LG), rows = 2u * p.nkv;
   for (uint32_t r0 = lane / LG; r0 < rows; r0 += RPW * U) {
-    float f[U][8];
+    if (r0 >= RPW * U) bring(r0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t r = r0 + u * RPW, h = r < p.nkv ? r : r - p.nkv;
-      if (r < rows && col < p.head_dim) {
-        load8<DT>(static_cast<const char*>(r < p.nkv ? k : v) +
-                      SZ * (token * stride + static_cast<uint64_t>(h) * p.head_dim + col),
-                  f[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[u][i] = 0.0f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t r = r0 + u * RPW, h = r < p.nkv ? r : r - p.nkv;
+      float f[8];
+      widen8<DT>(x[u], f);
       float scale = 0.0f;
       if constexpr (cache_codes<CT>()) {
         float a = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a = maximumf(a, __builtin_fabsf(f[u][i]));
+        for (int i = 0; i < 8; ++i) a = maximumf(a, __builtin_fabsf(f[i]));
 #pragma unroll
         for (int o = 1; o < LG; o <<= 1) a = maximumf(a, __shfl_xor(a, o));
         const bool some = a >= 1e-30f, fine = a < INFINITY;   // neither where a is NaN
         const float inv = some && fine ? cache_most<CT>() / a : 0.0f;
+        if (inv == 0.0f) {   // (codes of zero, not of minus zero)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = 0.0f;
+        }
         scale = fine ? (some ? a / cache_most<CT>() : 0.0f) : NAN;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[u][i] = inv != 0.0f ? f[u][i] * inv : 0.0f;
+        for (int i = 0; i < 8; ++i) {
+          f[i] *= inv;
+          asm("" : "+v"(f[i]));   // (rounded before the code is)
+        }
       }
       if (r < rows && col < p.head_dim) {
         void* pool = r < p.nkv ? p.k : p.v;
         const uint64_t at = pool_row(p, s, page, h, row) + col;
         if constexpr (cache_codes<CT>()) {
-          *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(pool) + at) = encode8<CT>(f[u]);
+          *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(pool) + at) = encode8<CT>(f);
           if (col == 0)
             (r < p.nkv ? p.k_scale : p.v_scale)[pool_scale(p, s, page, h, row)] = scale;
         } else {
-          store8<CT>(static_cast<uint16_t*>(pool) + at, f[u]);
+          store8<CT, false>(static_cast<uint16_t*>(pool) + at, f);
         }
       }
     }
@@ -226,7 +249,7 @@ kv_cache_read(PagedPool p, PagedSeqs s, void* __restrict__ k, void* __restrict__
             if constexpr (DT == kF16) asm("" : "+v"(f[kv][u][i]));
           }
         } else {
-          load8<CT>(static_cast<const uint16_t*>(pool) + at, f[kv][u]);
+          widen8<CT>(load8<CT>(static_cast<const uint16_t*>(pool) + at), f[kv][u]);
         }
       }
     }
@@ -239,8 +262,8 @@ kv_cache_read(PagedPool p, PagedSeqs s, void* __restrict__ k, void* __restrict__
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       void* out = kv ? v : k;
-      if constexpr (DT == kF32) store8<DT>(static_cast<float*>(out) + at, f[kv][u]);
-      else store8<DT>(static_cast<uint16_t*>(out) + at, f[kv][u]);
+      if constexpr (DT == kF32) store8<DT, true>(static_cast<float*>(out) + at, f[kv][u]);
+      else store8<DT, true>(static_cast<uint16_t*>(out) + at, f[kv][u]);
     }
   }
 }

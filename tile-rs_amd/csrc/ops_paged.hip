@@ -21,6 +21,9 @@ namespace {
 
 template <int N> using Int = std::integral_constant<int, N>;
 
+// Lanes that one launch can have.
+constexpr uint64_t kMostLanes = 0xffffffffu;
+
 bool codes(th_dtype d) { return d == TH_E4M3 || d == TH_I8; }
 
 // The structs' sizes and pointers; `need_rows`: the call has new tokens.
@@ -197,6 +200,8 @@ int th_kv_cache_write(const th_kv_pages* pages, const th_kv_batch* seqs, const v
   if (sq.batch == 0 || sq.total_q == 0) return TH_OK;
   if (stride > (uint64_t{1} << 60) / sq.total_q)
     return fail(TH_KERNEL_ERROR, "kv_cache_write: stride is too large");
+  if ((uint64_t{sq.total_q} + 3) / 4 * 256 > kMostLanes)
+    return fail(TH_KERNEL_ERROR, "kv_cache_write: grid too large");
   if (!k || !v) return fail(TH_KERNEL_ERROR, "kv_cache_write: null pointer");
   if (!aligned16(k) || !aligned16(v))
     return fail(TH_KERNEL_ERROR, "kv_cache_write: K and V must be 16-byte aligned");
@@ -224,10 +229,10 @@ int th_kv_cache_read(const th_kv_pages* pages, const th_kv_batch* seqs, void* k,
   int rc = TH_OK;
   by_float(dtype, [&](auto dt) {
     by_cache(pages->dtype, pool.head_dim, [&](auto ct, auto lg) {
-      constexpr uint32_t U = 4, per = U * 256 / lg.value;
+      constexpr uint32_t U = 2, per = U * 256 / lg.value;
       const uint32_t nchunks = (max_seq + per - 1) / per;
       const uint64_t rows = static_cast<uint64_t>(sq.batch) * pool.nkv;
-      if (rows > 0x7fffffffu / nchunks) {
+      if (rows * 256 > kMostLanes / nchunks) {
         rc = fail(TH_KERNEL_ERROR, "kv_cache_read: grid too large");
         return;
       }
@@ -284,7 +289,7 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
   a.group = num_heads / nkv;
   a.scale_log2 = th::kLog2e / std::sqrt(static_cast<float>(D));
   const AttnPlan plan = attn_plan(a.seqs, nkv, a.group, D);
-  if (plan.items * plan.parts > 0x7fffffffu)
+  if (plan.items * plan.parts * th::pgd::chunk::NT > kMostLanes)
     return fail(TH_KERNEL_ERROR, "attention_paged: grid too large");
   const size_t need = plan.rows_bytes + plan.chunk_bytes;
   th::ScratchHold hold;
