@@ -119,16 +119,20 @@ struct AttnPlan {
 // CUs of a whole MI355X, not of the current device, so that the workspace's size does not
 // depend on it.
 constexpr uint32_t kCus = 256;
-// Rows up to which a sequence stays with the rows' kernel.
-constexpr uint32_t kSplitRows = 64;
 
-AttnPlan attn_plan(const th::PagedSeqs& s, uint32_t nkv, uint32_t group, uint32_t head_dim) {
+AttnPlan attn_plan(const th::PagedSeqs& s, const th_kv_pages& pages, uint32_t group) {
+  const uint32_t nkv = pages.num_kv_heads, head_dim = pages.head_dim;
+  // Rows up to which a sequence stays with the rows' kernel, which widens codes once for a tile
+  // of 32 rows where the chunks' kernel does it for 256.  16 sequences of 2000 positions, 8 heads
+  // of 128, with 32, 64 and 96 rows for each head: bf16 44, 57, 90 us there, 43 at each size on
+  // the chunks' kernel; e4m3 38, 45, 66 there, 51 to 53 on the chunks' kernel.
+  const uint32_t split = codes(pages.dtype) ? 64 : 32;
   AttnPlan p;
   const uint32_t hd = head_width(head_dim);
   const uint64_t rows = static_cast<uint64_t>(s.total_q) * group;
   // a token per sequence: all of them steps, most likely
-  const bool chunks = hd <= 128 && rows > kSplitRows && s.total_q > s.batch;
-  p.split_rows = !chunks ? 0xffffffffu : s.batch == 1 ? 0u : kSplitRows;
+  const bool chunks = hd <= 128 && rows > split && s.total_q > s.batch;
+  p.split_rows = !chunks ? 0xffffffffu : s.batch == 1 ? 0u : split;
   if (p.split_rows != 0) {
     if (hd <= 128 && rows > 16ull * s.batch) p.tile_rows = 32;
     // at least the units of any lengths that the structs allow
@@ -253,7 +257,7 @@ size_t th_attention_paged_workspace_size(const th_kv_pages* pages, const th_kv_b
       num_heads == 0 || num_heads % pool.nkv != 0)
     return 0;   // (th_attention_paged refuses the same arguments)
   if (sq.batch == 0 || sq.total_q == 0) return 0;
-  const AttnPlan p = attn_plan(sq, pool.nkv, num_heads / pool.nkv, pool.head_dim);
+  const AttnPlan p = attn_plan(sq, *pages, num_heads / pool.nkv);
   return p.rows_bytes + p.chunk_bytes;
 }
 
@@ -288,7 +292,7 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
   a.nh = num_heads;
   a.group = num_heads / nkv;
   a.scale_log2 = th::kLog2e / std::sqrt(static_cast<float>(D));
-  const AttnPlan plan = attn_plan(a.seqs, nkv, a.group, D);
+  const AttnPlan plan = attn_plan(a.seqs, *pages, a.group);
   if (plan.items * plan.parts * th::pgd::chunk::NT > kMostLanes)
     return fail(TH_KERNEL_ERROR, "attention_paged: grid too large");
   const size_t need = plan.rows_bytes + plan.chunk_bytes;
