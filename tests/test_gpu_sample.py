@@ -34,13 +34,13 @@ def kept(x, temp, k, p, min_p):
 def plain(x, u, temp=1.0, k=0, p=1.0, min_p=0.0):
     """The token from 64 bits, and every token that 32-bit weights may give.  A weight is a power to
     base 2 of a product in f32 with its rounding put back, so good to 2^-21, and a mass to as much
-    of itself; the whole numbers of 2^-31 add half a step for each token: together `eps` of the
+    of itself; the whole numbers of 2^-40 add half a step for each token: together `eps` of the
     kept mass.  Tokens that a cut by mass or weight leaves out or keeps by less than that may be on
     its other side, which moves the masses by theirs."""
     order, w, keep = kept(x, temp, k, p, min_p)
     if order.size == 0:
         return -1, {-1}
-    eps = 2.0 ** -20 + w.size * 2.0 ** -32
+    eps = 2.0 ** -20 + w.size * 2.0 ** -41
     edge = np.zeros(w.size, bool)
     if min_p > 0:
         edge |= np.abs(w - min_p) < eps * min_p
@@ -114,6 +114,56 @@ def test_limits(dev, stream, dtype, rows, vocab):
         _, sure = check(dev, stream, x, dtype, rng.random(rows),
                         temperature=rng.uniform(0.4, 1.5, rows), **{n: make[n] for n in limits})
         assert sure >= rows - 1
+
+
+@pytest.mark.parametrize("dtype", [D.F32, D.BF16, D.F16])
+@pytest.mark.parametrize("rows", [1, 2, 130])
+def test_long_rows(dev, stream, dtype, rows):
+    """Few long rows without limits are spread over many workgroups, many are not: the same answers
+    at parts' borders, with masked parts, infinities, an empty row and any number."""
+    rng = np.random.default_rng(rows)
+    vocab = 70001
+    x = rng.standard_normal((rows, vocab)).astype(np.float32) * 3
+    x[0, :50000] = -np.inf if rows != 2 else np.nan
+    x[rows - 1, 60000:] = -np.inf
+    u = rng.random(rows)
+    check(dev, stream, pg.narrow(x, dtype), dtype, u, vocab + 1)
+    for end in (0.0, 1.0, 1 - 2.0 ** -24, -2.0, np.nan):
+        got = run(dev, stream, pg.narrow(x, dtype), dtype, np.full(rows, end))
+        for r in range(rows):
+            order, _, _ = kept(pg.widen(pg.narrow(x[r], dtype), dtype).astype(np.float64), 1.0, 0,
+                               1.0, 0.0)
+            if end == 1.0:
+                assert got[r] == order.max()
+            elif not end > 0:
+                assert got[r] == order.min()
+    one = np.full((rows, vocab), np.nan if rows == 2 else -np.inf, np.float32)
+    y = pg.narrow(one, dtype)
+    assert (run(dev, stream, y, dtype, u) == -1).all()
+    one[:, 65000] = -np.float32(np.finfo(np.float16).max)
+    y = pg.narrow(one, dtype)
+    assert (run(dev, stream, y, dtype, u) == 65000).all()
+    z = x.copy()
+    z[:, [10, 69999]] = np.inf
+    got = run(dev, stream, pg.narrow(z, dtype), dtype, np.where(np.arange(rows) % 2, 0.7, 0.3))
+    assert np.array_equal(got, np.where(np.arange(rows) % 2, 69999, 10))
+    cold = run(dev, stream, pg.narrow(x, dtype), dtype, u, temperature=np.zeros(rows))
+    assert np.array_equal(cold, [kept(pg.widen(pg.narrow(r, dtype), dtype).astype(np.float64), 0.0,
+                                      0, 1.0, 0.0)[0][0] for r in x])
+
+
+@pytest.mark.parametrize("vocab", [170001, 300000])
+def test_rows_past_the_registers(dev, stream, vocab):
+    """Rows that do not stay in registers, with limits and wide ranges of equal logits."""
+    rng = np.random.default_rng(vocab)
+    x = pg.narrow(rng.standard_normal((6, vocab)) * 2, D.BF16)
+    _, sure = check(dev, stream, x, D.BF16, rng.random(6), top_k=np.array([5, 4000, 100000, 0, 1, 50]),
+                    top_p=np.array([0.9, 0.5, 0.99, 0.3, 1.0, 0.0]))
+    assert sure >= 5
+    x = rng.standard_normal((6, vocab)).astype(np.float32)
+    _, sure = check(dev, stream, x, D.F32, rng.random(6), vocab + 3,
+                    temperature=rng.uniform(0.5, 1.5, 6), min_p=rng.uniform(0, 0.3, 6))
+    assert sure >= 5
 
 
 def test_counts_are_exact(dev, stream):
