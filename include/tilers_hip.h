@@ -307,15 +307,15 @@ int th_kv_cache_write(const th_kv_pages* pages, const th_kv_batch* seqs, const v
 
 /* Read positions [0, kv_len[b]) of every sequence into K and V,
  * [batch][num_kv_heads][max_seq][head_dim] in dtype (F32, F16 or BF16; code * scale is rounded
- * to f32, then to dtype), the layout of th_attention_prefill and th_attention_decode.  Positions from max_seq on are not read, rows
- * from kv_len[b] on are left as they were. */
+ * to f32, then to dtype), the layout of th_attention_prefill and th_attention_decode.  Positions
+ * from max_seq on are not read, rows from kv_len[b] on are left as they were. */
 int th_kv_cache_read(const th_kv_pages* pages, const th_kv_batch* seqs, void* k, void* v,
                      uint32_t max_seq, th_dtype dtype, th_stream s);
 
 /* Causal attention of the new tokens over their sequences' pages: the token at position p sees
  * positions 0 .. p, its own K and V among them (write them first).  Q is
  * [total_q][num_heads][head_dim] with q_stride elements between tokens (0: dense; else at least
- * num_heads * head_dim and a multiple of 8), O the same, dense.  dtype is F16 or BF16; the cache
+ * num_heads * head_dim and a multiple of 8), O the same, dense, and not in Q's memory.  dtype is F16 or BF16; the cache
  * is of that dtype, or E4M3 or I8.  num_heads is a multiple of num_kv_heads.  Scores, softmax
  * and sums are f32; probabilities are rounded to dtype.  A token that sees nothing gives zeros.
  * What a token does not see has no effect on it, NaN and infinities included.
@@ -339,10 +339,14 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
  * less than top_p of it before it (all where top_p >= 1 or NaN); of those the ones with
  * w_i >= min_p; and always the first.  tokens[row] is the lowest index whose mass, with that of
  * the kept ones of lower index, exceeds uniform * (mass of the kept).  Where temperature is <= 0
- * or NaN that is the first of the order.  Logits of NaN and -infinity are never chosen; a row of nothing
- * else gives -1.  Weights are f32 with steps of 2^-31 of the largest; masses are exact sums of
- * them, so a result does not depend on the order of summation.  Cf. the reference's
- * __tile_sample_top_p intrinsic, which its emitters print and this runtime takes no tile for. */
+ * or NaN that is the first of the order.  Logits of NaN and -infinity are never chosen; a row of
+ * nothing else gives -1.  vocab is at most 2^23.  Weights are f32 in steps of 2^-40 of the largest and masses exact sums
+ * of them.  Long rows without top_k, top_p and min_p may be divided: each part then has its own
+ * largest weight and the parts' masses are joined in f64, on the stream's scratch.  A captured
+ * call is never divided, so it may choose otherwise than an eager one, but only where uniform
+ * lies within 2^-19 of a border between two tokens; calls alike give the same token.  Cf. the
+ * reference's __tile_sample_top_p intrinsic, which its emitters print and this runtime takes no
+ * tile for. */
 int th_sample(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab, uint64_t stride,
               th_dtype dtype, const float* uniform, const float* temperature,
               const int32_t* top_k, const float* top_p, const float* min_p, th_stream s);

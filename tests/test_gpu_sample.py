@@ -137,6 +137,9 @@ def test_long_rows(dev, stream, dtype, rows):
                 assert got[r] == order.max()
             elif not end > 0:
                 assert got[r] == order.min()
+    flat = pg.narrow(np.full((rows, vocab), 3.5), dtype)
+    assert (run(dev, stream, flat, dtype, np.ones(rows)) == vocab - 1).all()
+    assert (run(dev, stream, flat, dtype, np.zeros(rows)) == 0).all()
     one = np.full((rows, vocab), np.nan if rows == 2 else -np.inf, np.float32)
     y = pg.narrow(one, dtype)
     assert (run(dev, stream, y, dtype, u) == -1).all()
@@ -164,6 +167,19 @@ def test_rows_past_the_registers(dev, stream, vocab):
     _, sure = check(dev, stream, x, D.F32, rng.random(6), vocab + 3,
                     temperature=rng.uniform(0.5, 1.5, 6), min_p=rng.uniform(0, 0.3, 6))
     assert sure >= 5
+    x = rng.standard_normal((3, 4 * vocab + 1)).astype(np.float32)   # hundreds of parts
+    _, sure = check(dev, stream, x, D.F32, [0.001, 0.4, 0.9995], temperature=[0.5, 1.0, 2.0])
+    assert sure == 3
+
+
+@pytest.mark.parametrize("limits", [{}, dict(top_k=[0] * 3), dict(top_p=[1.0] * 3)])
+@pytest.mark.parametrize("vocab", [9000, 40000, 1 << 20, 1 << 23])
+def test_masses_past_53_bits(dev, stream, vocab, limits):
+    """All alike: sums of that many weights of 1 in steps of 2^-40, to the first, a middle and the
+    last token."""
+    x = pg.narrow(np.zeros((3, vocab)), D.BF16)
+    got = run(dev, stream, x, D.BF16, [0.0, 0.5, 1.0], **limits)
+    assert got.tolist() == [0, vocab // 2, vocab - 1]
 
 
 def test_counts_are_exact(dev, stream):

@@ -147,8 +147,10 @@ def test_sample_refusals():
     refused("stride is less", a, a, 2, 10, D.F32, a, stride=9)
     refused("stride is too large", a, a, 2, 10, D.F32, a, stride=1 << 60)
     refused("vocab == 0", a, a, 2, 0, D.F32, a)
-    refused("below 2^31", a, a, 2, 1 << 31, D.F32, a)
+    refused("at most 2^23", a, a, 2, (1 << 23) + 1, D.F32, a)
+    refused("at most 2^23", a, a, 2, 1 << 31, D.F32, a)
     refused("below 2^31", a, a, 1 << 31, 2, D.F32, a)
+    refused("grid too large", a, a, 1 << 22, 2, D.F32, a)
     for i in range(3):
         p = [a, a, a]
         p[i] = 0

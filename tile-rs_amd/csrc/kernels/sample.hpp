@@ -2,7 +2,7 @@
 // random number.
 //
 //   w_i = exp((x_i - x_max) / T) in f32, held as a whole number of 2^-40, so that masses are
-//   exact in 64 bits and no order of summation shows.
+//   exact in 64 bits (up to 2^23 logits of weight 1) and no order of summation shows.
 //
 // The kept set is a prefix of the order (x falling, then index rising), so each limit is a cut:
 // a (key, index) pair, the last one kept, with `key` the order-preserving whole number of x.  A
@@ -361,6 +361,13 @@ struct Sampler {
   }
 };
 
+// A value that the f64 of a mass exceeds, for numbers of 1 and more: the last step of it, or past
+// 2^53, where steps no longer show, a rounding.
+__device__ __forceinline__ double short_of(uint64_t mass) {
+  const double m = static_cast<double>(mass);
+  return min(m - 1.0, m * (1.0 - 0x1p-52));
+}
+
 // The first element of blocks [k0, k1) at which the mass from `before` on exceeds `target`, which
 // lies in them.  A long range is divided among the waves, and the share that holds the place
 // divided again, down to a block per thread.  kept(index, logit): an element's mass.
@@ -511,8 +518,8 @@ sample_rows(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
   __syncthreads();
   uint64_t all = 0, before = 0;
   for (int i = 0; i < NW; ++i) all += sh.wave_a[i];
-  const double target = min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0,
-                            static_cast<double>(all) - 0.5);
+  const double target =
+      min(u > 0.0f ? static_cast<double>(u) * static_cast<double>(all) : 0.0, short_of(all));
   uint32_t w = 0;
   while (w < NW - 1 && static_cast<double>(before + sh.wave_a[w]) <= target)
     before += sh.wave_a[w++];
@@ -623,18 +630,21 @@ sample_pick(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
   }
   const double target =
       greedy || !(u > 0.0f) ? 0.0 : min(static_cast<double>(u) * all, all * (1.0 - 0x1p-52));
-  double before = 0.0;
+  // (A lane's sum is of its own order: the last part's may round to below `all`, and is taken then
+  // where none is above the target.)
+  double before = 0.0, below = 0.0;
   uint32_t part = 0;
   for (base = 0; base < parts; base += 64) {
     if (parts > 64) sum64(base);
-    const uint64_t in = __builtin_amdgcn_ballot_w64(mass > 0.0 && before + upto > target);
-    if (in != 0) {
-      const int l = __builtin_ctzll(in);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(mass > 0.0);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(mass > 0.0 && below + upto > target);
+    if (some != 0) {
+      const int l = in != 0 ? __builtin_ctzll(in) : 63 - __builtin_clzll(some);
       part = base + l;
-      before += __shfl(upto - mass, l);
-      break;
+      before = below + __shfl(upto - mass, l);
     }
-    before += __shfl(upto, 63);
+    if (in != 0) break;
+    below += __shfl(upto, 63);
   }
   const float part_top = sums[part].top;
   const double f = factor(part_top);
@@ -656,7 +666,7 @@ sample_pick(const void* __restrict__ logits, int32_t* __restrict__ tokens, uint3
   }
   const Weigher weigh = Weigher::make(part_top, temp);
   const double local =
-      max(0.0, min((target - before) / f, static_cast<double>(sums[part].mass) - 0.5));
+      max(0.0, min((target - before) / f, short_of(sums[part].mass)));
   find_place(sh, blocks, k0, k1, 0, local, [&](uint32_t, float x) { return weigh(x); },
              tokens + r);
 }
