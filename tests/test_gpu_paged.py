@@ -163,21 +163,25 @@ def test_read_past_the_table(dev, stream):
 # ---- attention -----------------------------------------------------------------------------
 
 def bound(o, mean, reach, dtype, head_dim, held, codes):
-    """How far O may be from 64 bits.  With u half a step of dtype: the probabilities' rounding
-    moves the weighted mean by at most u sum p |v|, O's own by u |o|.  A score is a sum of D exact
-    products in f32 (D 2^-24 sum |q k| at most), scaled twice and subtracted (4 roundings of a
-    value of at most 2 reach log2 e), then a power to base 2 good to 2^-21: weights are off by e
-    each, which moves numerator and denominator by as much.  Sums over the positions: held
-    roundings of 2^-24 at most, in parts of 8, so 2^-24 (held / 8 + 64).  f16 probabilities below
-    2^-14 are multiples of 2^-24 and the largest is at least 1 (or 1/2 with codes, whose scales
-    are relative to a power of two within a factor of two of the largest; values at most that
-    factor, 2, times the largest), a position's error 2^-25 of the largest value."""
+    """How far O may be from 64 bits.  Half a step of a type is u.  O's own rounding: u |o|.  The
+    weights' rounding, to dtype or with codes to f16: up sum p |v| at most in the product with V;
+    without codes the sum is of the rounded ones too, so the weighted mean moves by
+    |sum p e (v - o)| <= up (sum p |v| + |o|).  A score is a sum of D exact products in f32
+    (D 2^-24 sum |q k| at most), scaled twice and subtracted (4 roundings of a value of at most 2
+    reach log2 e), then a power to base 2 good to 2^-21: weights are off by e each, which moves
+    numerator and denominator by as much.  Sums over the positions: held roundings of 2^-24 at
+    most, in parts of 8, so 2^-24 (held / 8 + 64).  f16 weights below 2^-14 are multiples of 2^-24
+    and the largest is at least 1 (or 1/2 with codes, whose scales are relative to a power of two
+    within a factor of two of the largest; values at most that factor, 2, times the largest), a
+    position's error 2^-25 of the largest value."""
     u = pg.HALF[dtype]
+    up = pg.HALF[D.F16] if codes else u
     e = (head_dim + 8) * 2.0 ** -23 * reach[..., None] + 2.0 ** -20 + 2.0 ** -24 * (held / 8 + 64)
-    tol = u * (mean + np.abs(o)) * 1.01 + 2 * e * mean + 1e-30
+    tol = (up * (mean + (0 if codes else np.abs(o))) + u * np.abs(o)) * 1.01 + 2 * e * mean + 1e-30
+    if dtype == D.F16 or codes:
+        tol = tol + held * 2.0 ** -24 * (4 if codes else 1) * max(1.0, float(np.abs(mean).max()))
     if dtype == D.F16:
-        tol = tol + held * 2.0 ** -24 * (4 if codes else 1) * max(1.0, float(np.abs(mean).max())) \
-            + 2.0 ** -25
+        tol = tol + 2.0 ** -25
     return tol
 
 
@@ -292,29 +296,31 @@ def test_peaked(dev, stream, dtype, cache):
 
 
 @pytest.mark.parametrize("cache", [D.E4M3, D.I8])
-@pytest.mark.parametrize("peak", [1e-6, 3e3])
-def test_scales_far_from_one_in_f16(dev, stream, cache, peak):
-    """f16 Q beside scales whose products with probabilities leave f16's range: V alone is scaled
-    (K keeps scores of order one), and grows by the position."""
+@pytest.mark.parametrize("dtype,peak", [(D.F16, 1e-6), (D.F16, 3e3), (D.BF16, 1e-27),
+                                        (D.BF16, 1e-6), (D.BF16, 1e20), (D.BF16, 3e28),
+                                        (D.BF16, 1e35)])
+def test_scales_far_from_one(dev, stream, cache, dtype, peak):
+    """Scales whose products with probabilities leave f16's range, and f32's with the largest taken
+    out: V alone is scaled (K keeps scores of order one), at random by the position."""
     rng = np.random.default_rng(12)
     length, new = [300, 50], [1, 20]
-    pool, table, start, q = make(rng, cache, D.F16, 1, 4, 64, 16, length, new)
+    pool, table, start, q = make(rng, cache, dtype, 1, 4, 64, 16, length, new)
     grow = np.float32(peak) * np.exp2(rng.uniform(-6, 3, pool.scale[1].shape)).astype(np.float32)
     pool.scale[1] = pool.scale[1] * grow
-    got = run_attention(dev, stream, pool, table, start, length, q, D.F16, 4)
+    got = run_attention(dev, stream, pool, table, start, length, q, dtype, 4)
     for b, n in enumerate(length):
         rows = slice(start[b], start[b + 1])
         kv = [pool.read(i, table[b], n) for i in range(2)]
-        o, mean, reach = pg.attention(pg.widen(q[rows], D.F16).astype(np.float64), kv,
+        o, mean, reach = pg.attention(pg.widen(q[rows], dtype).astype(np.float64), kv,
                                       pool.there(table[b], n), new[b], n, 4)
         e = (64 + 8) * 2.0 ** -23 * reach[..., None] + 2.0 ** -20 + 2.0 ** -24 * (n / 8 + 64)
         # probabilities times scales are multiples of 2^-24 of a power of two of at most the
         # largest scale; codes reach 448 (127); O's own step is absolute below 2^-14
         most = float(pool.scale[1][table[b][:-(-n // 16)]][~np.isnan(
             pool.scale[1][table[b][:-(-n // 16)]])].max())
-        tol = (2.0 ** -11 * (mean + np.abs(o)) * 1.01 + 2 * e * mean + 2.0 ** -25
-               + n * 2.0 ** -24 * most * pg.MOST[cache])
-        assert (np.abs(pg.widen(got[rows], D.F16) - o) <= tol).all()
+        tol = ((2.0 ** -11 * mean + pg.HALF[dtype] * np.abs(o)) * 1.01 + 2 * e * mean
+               + (2.0 ** -25 if dtype == D.F16 else 0) + n * 2.0 ** -24 * most * pg.MOST[cache])
+        assert (np.abs(pg.widen(got[rows], dtype) - o) <= tol).all()
 
 
 @pytest.mark.parametrize("dtype,cache", TYPES)

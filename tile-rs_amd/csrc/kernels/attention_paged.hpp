@@ -30,6 +30,22 @@ __device__ __forceinline__ uint32_t pack2h(float lo, float hi) {
   }
 }
 
+// a + x + y of a pair as pack2h rounded it.  (Weights are summed as the product with V takes them,
+// so that the mean is one of weights that sum to 1: a token that has all the weight gives its
+// values exactly.)
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t xy, float a) {
+  if constexpr (DT == kBF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, xy),
+                                           __builtin_bit_cast(b2, 0x3f803f80u), a, false);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, xy), __builtin_bit_cast(h2, 0x3c003c00u),
+                                  a, false);
+  }
+}
+
 // Four codes -> four values of type DT, exactly.
 template <int DT, int CT>
 __device__ __forceinline__ u32x2 widen4(uint32_t w) {
@@ -106,7 +122,9 @@ __device__ __forceinline__ int32_t paged_checked(const PagedSeqs& s, int32_t id)
 // are taken relative to its maximum plus the exponent of the largest scale that it has seen (at
 // least kLeastExp, so that f32 holds the rest): products are then at most 2^8 as without scales,
 // and numerator and denominator share the factor.
-constexpr float kLeastExp = -100.0f;
+// (Weights end at 2^-126 of f32: from exponents of kMostExp on they would lose what is 2^-36 of
+// the largest and less, and a tile that sees such a scale is summed again by SlowRow.)
+constexpr float kLeastExp = -100.0f, kMostExp = 90.0f;
 __device__ __forceinline__ float scale_exp(float most) {
   return most > 0.0f ? static_cast<float>(__builtin_amdgcn_frexp_expf(most)) : kLeastExp;
 }
@@ -343,7 +361,9 @@ struct SlowRow {
 template <int DT, int CT, int HD, int MT>
 struct RowsTile {
   static constexpr bool kCodes = cache_codes<CT>();
-  static constexpr bool kExps = kCodes && DT == kF16;   // (scale_exp)
+  // Weights times codes' scales, and the codes of V, which f16 holds exactly, go into the product
+  // as f16 whatever Q is: 8 times less rounding than bf16, at 0 to 4% of the time.
+  static constexpr int PT = kCodes ? static_cast<int>(kF16) : DT;
   static constexpr int ESZ = cache_size<CT>();
   static constexpr int TR = 16 * MT;
   static constexpr int NS = HD / 32;             // K fragments (32 values deep) of a position
@@ -441,9 +461,9 @@ struct RowsTile {
       const uint32_t r = i * (32 / VL) + lane / VROW, c = lane % VROW;
       const u32x4 w = st.v[i];
       if constexpr (kCodes) {
-        const u32x2 a = widen4<DT, CT>(w[0]), b = widen4<DT, CT>(w[1]);
+        const u32x2 a = widen4<PT, CT>(w[0]), b = widen4<PT, CT>(w[1]);
         *reinterpret_cast<u32x4*>(lds + vaddr(r, 2 * c)) = u32x4{a[0], a[1], b[0], b[1]};
-        const u32x2 d = widen4<DT, CT>(w[2]), e = widen4<DT, CT>(w[3]);
+        const u32x2 d = widen4<PT, CT>(w[2]), e = widen4<PT, CT>(w[3]);
         *reinterpret_cast<u32x4*>(lds + vaddr(r, 2 * c + 1)) = u32x4{d[0], d[1], e[0], e[1]};
       } else {
         *reinterpret_cast<u32x4*>(lds + vaddr(r, c)) = w;
@@ -469,7 +489,7 @@ struct RowsTile {
       const u32x2 hi = lds::read_tr16(lds + vaddr(16 + r, ch) + in);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
-        y.acc[i][c] = mfma16x16x32<DT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[i], y.acc[i][c]);
+        y.acc[i][c] = mfma16x16x32<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[i], y.acc[i][c]);
     }
   }
 
@@ -519,7 +539,7 @@ struct RowsTile {
       for (int x = 0; x < NC; ++x) y.acc[i][x] = f32x4{0, 0, 0, 0};
       y.m[i] = -INFINITY;
       y.l[i] = 0.0f;
-      y.ev[i] = kExps ? kLeastExp : 0.0f;
+      y.ev[i] = kCodes ? kLeastExp : 0.0f;
     }
     char* const vlds = arena + wave * WB;
     bool odd = false;   // NaN or infinities in V near the rows' ends
@@ -591,21 +611,19 @@ struct RowsTile {
 #pragma unroll
             for (int x = 0; x < 8; ++x) w[x] = (x & 3) < lim[x >> 2] ? vs[x] : 0.0f;
           }
-          if constexpr (kExps) {
-            float most = w[0];
+          float most = w[0];
 #pragma unroll
-            for (int x = 1; x < 8; ++x) most = fmaxf(most, w[x]);
-            big = scale_exp(most);
-          }
+          for (int x = 1; x < 8; ++x) most = fmaxf(most, w[x]);
+          big = scale_exp(most);
         }
         float alpha = 1.0f;
         bool moved = false;
-        if (__builtin_amdgcn_ballot_w64(mx > y.m[i] + 8.0f || (kExps && big > y.ev[i])) != 0) {
+        if (__builtin_amdgcn_ballot_w64(mx > y.m[i] + 8.0f || (kCodes && big > y.ev[i])) != 0) {
           mx = fmaxf(mx, __shfl_xor(mx, 16));
           mx = fmaxf(mx, __shfl_xor(mx, 32));
           const float old = y.m[i] + y.ev[i];
           y.m[i] = fmaxf(y.m[i], mx);
-          if constexpr (kExps) {
+          if constexpr (kCodes) {
             big = fmaxf(big, __shfl_xor(big, 16));
             y.ev[i] = fmaxf(y.ev[i], fmaxf(big, __shfl_xor(big, 32)));
           }
@@ -618,8 +636,10 @@ struct RowsTile {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           p[x] = exp2_fast(s[i][x >> 2][x & 3] - mu);
-          y.l[i] += p[x];
-          if constexpr (kCodes) p[x] *= w[x];
+          if constexpr (kCodes) {
+            y.l[i] += p[x];
+            p[x] *= w[x];
+          }
         }
         if (moved) {
 #pragma unroll
@@ -627,8 +647,12 @@ struct RowsTile {
 #pragma unroll
             for (int j = 0; j < 4; ++j) y.acc[i][x][j] *= alpha;
         }
-        pf[i] = u32x4{pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
-                      pack2h<DT>(p[6], p[7])};
+        pf[i] = u32x4{pack2h<PT>(p[0], p[1]), pack2h<PT>(p[2], p[3]), pack2h<PT>(p[4], p[5]),
+                      pack2h<PT>(p[6], p[7])};
+        if constexpr (!kCodes) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) y.l[i] = add_pair<DT>(pf[i][x], y.l[i]);
+        }
       }
       pv(vlds, pf, y);
     }
@@ -637,7 +661,10 @@ struct RowsTile {
     __shared__ float sm[4][TR], sl[4][TR];
     __shared__ uint32_t odds[4];
     lds_order();
-    const bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max;
+    bool any_odd = __builtin_amdgcn_ballot_w64(odd) != 0 && vis_min < vis_max;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      any_odd |= kCodes && __builtin_amdgcn_ballot_w64(y.ev[i] > kMostExp) != 0;
     if (lane == 0) odds[wave] = any_odd;
     float* wo = reinterpret_cast<float*>(vlds);
 #pragma unroll
@@ -859,7 +886,7 @@ struct ChunkTile {
   static_assert(HD == 64 || HD == 128, "chunk kernel head dim");
   static constexpr bool kCodes = cache_codes<CT>();
   static constexpr int ESZ = cache_size<CT>();
-  static constexpr bool kExps = kCodes && DT == kF16;   // (scale_exp)
+  static constexpr int PT = kCodes ? static_cast<int>(kF16) : DT;   // (RowsTile)
   static constexpr int RB = HD * 2;                  // bytes of a row in LDS
   static constexpr int KBYTES = chunk::KB * RB;      // of a block's K (or V)
   static constexpr int CPR = HD * ESZ / 16;          // 16-byte pieces of a row in memory
@@ -999,7 +1026,7 @@ attn_paged_chunk(AttnArgs a) {
   for (int i = 0; i < T::NDT; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-  float m = -INFINITY, l = 0.0f, ev = T::kExps ? kLeastExp : 0.0f;
+  float m = -INFINITY, l = 0.0f, ev = T::kCodes ? kLeastExp : 0.0f;
   if (t == 0) sh.odd = 0;
 
   // this thread's pieces of a block: rows xr, 16-byte pieces xc.  A wave's rows, from wr on, lie
@@ -1064,7 +1091,7 @@ attn_paged_chunk(AttnArgs a) {
         for (int x = 0; x < 2; ++x) {
           const u32x2 k0 = widen4<DT, CT>(k[2 * x]), k1 = widen4<DT, CT>(k[2 * x + 1]);
           *reinterpret_cast<u32x4*>(kl + T::kaddr(r, 2 * cc + x)) = u32x4{k0[0], k0[1], k1[0], k1[1]};
-          const u32x2 v0 = widen4<DT, CT>(v[2 * x]), v1 = widen4<DT, CT>(v[2 * x + 1]);
+          const u32x2 v0 = widen4<T::PT, CT>(v[2 * x]), v1 = widen4<T::PT, CT>(v[2 * x + 1]);
           *reinterpret_cast<u32x4*>(vl + T::vaddr(r, 2 * cc + x)) = u32x4{v0[0], v0[1], v1[0], v1[1]};
         }
       } else {
@@ -1075,12 +1102,10 @@ attn_paged_chunk(AttnArgs a) {
     }
     if constexpr (T::kCodes) {
       if (t < 2 * KB) (t < KB ? sh.ks : sh.vs)[slot(j)][t & (KB - 1)] = st.scale;
-      if constexpr (T::kExps) {
-        if (wave == 1) {   // (its lanes hold all of vs)
-          static_assert(KB == 64, "vs in one wave");
-          const float most = wave_max(st.scale);
-          if (lane == 0) sh.big[slot(j)] = scale_exp(most);
-        }
+      if (wave == 1) {   // (its lanes hold all of vs)
+        static_assert(KB == 64, "vs in one wave");
+        const float most = wave_max(st.scale);
+        if (lane == 0) sh.big[slot(j)] = scale_exp(most);
       }
     }
     if (odd && (j + 1) * KB > tile_min) sh.odd = 1;   // (from any thread: one value)
@@ -1131,7 +1156,7 @@ attn_paged_chunk(AttnArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       const u32x4 f = frag[i % (AHEAD + 1)];
       if constexpr (Q) s[i % NKT] = mfma32x32x16<DT>(f, qf[i / NKT], s[i % NKT]);
-      else acc[i % T::NDT] = mfma32x32x16<DT>(f, pf[i / T::NDT], acc[i % T::NDT]);
+      else acc[i % T::NDT] = mfma32x32x16<T::PT>(f, pf[i / T::NDT], acc[i % T::NDT]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -1171,7 +1196,7 @@ attn_paged_chunk(AttnArgs a) {
     for (int q = 1; q < NSP; ++q) mx[0] = fmaxf(mx[0], mx[q]);
     const float top = pair_max(mx[0]) * a.scale_log2;
     float big = kLeastExp;
-    if constexpr (T::kExps) {
+    if constexpr (T::kCodes) {
       if (hides) {
         float most = 0.0f;
 #pragma unroll
@@ -1184,10 +1209,10 @@ attn_paged_chunk(AttnArgs a) {
         big = sh.big[at_ring];
       }
     }
-    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || (T::kExps && big > ev)) != 0) {
+    if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || (T::kCodes && big > ev)) != 0) {
       const float old = m + ev;
       m = fmaxf(m, top);
-      ev = T::kExps ? fmaxf(ev, big) : 0.0f;
+      ev = T::kCodes ? fmaxf(ev, big) : 0.0f;
       const float alpha = m == -INFINITY ? 1.0f : exp2_fast(old - (m + ev));
       l *= alpha;
 #pragma unroll
@@ -1203,7 +1228,7 @@ attn_paged_chunk(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] = exp2_fast(__builtin_fmaf(s[sp >> 1][8 * (sp & 1) + i], a.scale_log2, -mu));
-        (i & 1 ? l1 : l0) += p[i];
+        if constexpr (T::kCodes) (i & 1 ? l1 : l0) += p[i];
       }
       if constexpr (T::kCodes) {
 #pragma unroll
@@ -1217,8 +1242,12 @@ attn_paged_chunk(AttnArgs a) {
           }
         }
       }
-      pf[sp] = u32x4{pack2h<DT>(p[0], p[1]), pack2h<DT>(p[2], p[3]), pack2h<DT>(p[4], p[5]),
-                     pack2h<DT>(p[6], p[7])};
+      pf[sp] = u32x4{pack2h<T::PT>(p[0], p[1]), pack2h<T::PT>(p[2], p[3]),
+                     pack2h<T::PT>(p[4], p[5]), pack2h<T::PT>(p[6], p[7])};
+      if constexpr (!T::kCodes) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) (i & 1 ? l1 : l0) = add_pair<DT>(pf[sp][i], i & 1 ? l1 : l0);
+      }
     }
     l += l0 + l1;
   };
@@ -1261,7 +1290,8 @@ attn_paged_chunk(AttnArgs a) {
   auto record = [&](uint64_t at) {
     return a.chunk_ws + (static_cast<uint64_t>(part) * a.seqs.total_q * a.nh + at) * rec(HD);
   };
-  if (j0 < j1 && __builtin_amdgcn_readfirstlane(sh.odd) != 0) {   // (set before the last turn)
+  if (j0 < j1 && (__builtin_amdgcn_readfirstlane(sh.odd) != 0 ||   // (set before the last turn)
+                  (T::kCodes && __builtin_amdgcn_ballot_w64(ev > kMostExp) != 0))) {
     for (uint32_t r = wr0; r < min(nrows, wr0 + 32); ++r) {
       SlowRow<DT, CT, HD> y(a, c, b, h, r, j0 * KB, j1 * KB);
       const uint64_t at = (c.first + r / G) * static_cast<uint64_t>(a.nh) + h * G + r % G;
