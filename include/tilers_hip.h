@@ -315,10 +315,11 @@ int th_kv_cache_read(const th_kv_pages* pages, const th_kv_batch* seqs, void* k,
 /* Causal attention of the new tokens over their sequences' pages: the token at position p sees
  * positions 0 .. p, its own K and V among them (write them first).  Q is
  * [total_q][num_heads][head_dim] with q_stride elements between tokens (0: dense; else at least
- * num_heads * head_dim and a multiple of 8), O the same, dense, and not in Q's memory.  dtype is F16 or BF16; the cache
- * is of that dtype, or E4M3 or I8.  num_heads is a multiple of num_kv_heads.  Scores, softmax
- * and sums are f32; weights are rounded to dtype, with an 8-bit cache weight times scale to f16.  A token that sees nothing gives zeros.
- * What a token does not see has no effect on it, NaN and infinities included.
+ * num_heads * head_dim and a multiple of 8), O the same, dense, and not in Q's memory.  dtype is
+ * F16 or BF16; the cache is of that dtype, or E4M3 or I8.  num_heads is a multiple of
+ * num_kv_heads.  Scores, softmax and sums are f32; weights are rounded to dtype, with an 8-bit
+ * cache weight times scale to f16.  A token that sees nothing gives zeros.  What a token does not
+ * see has no effect on it, NaN and infinities included.
  * The work is split by the lengths on the device, so one captured call serves any lengths; the
  * parts' sums go to `workspace`, device memory of at least th_attention_paged_workspace_size
  * bytes for the same arguments (of the structs' sizes, not the lengths).  With NULL they go to
@@ -340,8 +341,8 @@ int th_attention_paged(const void* q, const th_kv_pages* pages, const th_kv_batc
  * w_i >= min_p; and always the first.  tokens[row] is the lowest index whose mass, with that of
  * the kept ones of lower index, exceeds uniform * (mass of the kept).  Where temperature is <= 0
  * or NaN that is the first of the order.  Logits of NaN and -infinity are never chosen; a row of
- * nothing else gives -1.  vocab is at most 2^23.  Weights are f32 in steps of 2^-40 of the largest and masses exact sums
- * of them.  Long rows without top_k, top_p and min_p may be divided: each part then has its own
+ * nothing else gives -1.  vocab is at most 2^23.  Weights are f32 in steps of 2^-40 of the
+ * largest and masses exact sums of them.  Long rows without top_k, top_p and min_p may be divided: each part then has its own
  * largest weight and the parts' masses are joined in f64, on the stream's scratch.  A captured
  * call is never divided, so it may choose otherwise than an eager one, but only where uniform
  * lies within 2^-19 of a border between two tokens; calls alike give the same token.  Cf. the

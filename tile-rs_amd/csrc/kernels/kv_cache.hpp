@@ -8,6 +8,12 @@
 //
 // A row (one token and head of K or V) is `LG` lanes of eight values: 16 bytes of a 16-bit
 // tensor per lane, and the row's maximum takes log2(LG) lane exchanges.
+//
+// Measured, 8 heads of 128: writing 25663 tokens of bf16 as i8 30 us (159 MB, 5.3 TB/s; 34 with
+// the loads behind the lookup of the page and the codes gathered by shifts), 56 tokens 4.6;
+// reading 8 sequences of up to 8192 positions from e4m3 into bf16 46 us (311 MB, 6.7 TB/s, a
+// third of it found in the last-level cache; 65 where nothing is), 77 with stores that go through
+// the caches and four rows in flight per lane instead of two, 118 with eight.
 #pragma once
 
 #include "common.hpp"
