@@ -250,7 +250,8 @@ TYPES = [(D.BF16, D.BF16), (D.F16, D.F16), (D.BF16, D.E4M3), (D.F16, D.E4M3), (D
 @pytest.mark.parametrize("dtype,cache", TYPES)
 @pytest.mark.parametrize("heads,group,head_dim,page", [
     (2, 4, 128, 16), (1, 1, 64, 32), (2, 8, 64, 16), (1, 7, 128, 64), (3, 1, 80, 16),
-    (1, 16, 32, 16), (1, 20, 48, 16), (1, 2, 256, 32), (1, 3, 144, 16),
+    (1, 16, 32, 16), (1, 20, 48, 16), (1, 2, 256, 32), (1, 3, 144, 16), (2, 2, 16, 16),
+    (1, 71, 64, 16), (1, 3, 112, 64), (1, 5, 208, 16),
 ])
 def test_steps(dev, stream, dtype, cache, heads, group, head_dim, page):
     """Single tokens: from one position to several hundred, pages that end inside a tile."""
@@ -404,6 +405,16 @@ def test_many_chunks(dev, stream, batch):
            for b, (n, x) in enumerate(zip(length, rng.integers(0, 200, batch)))]
     pool, table, start, q = make(rng, D.E4M3, D.F16, 1, 4, 64, 16, length, new)
     check_attention(dev, stream, pool, table, start, length, q, D.F16, 4)
+
+
+@pytest.mark.parametrize("batch", [1, 3, 70])
+def test_nobody_has_new_tokens(dev, stream, batch):
+    """Rows that belong to no sequence, behind sequences of many positions and of none."""
+    rng = np.random.default_rng(batch)
+    length = [900] + [0, 17] * (batch // 2)
+    length = (length + [5])[:batch]
+    pool, table, start, q = make(rng, D.BF16, D.BF16, 1, 4, 64, 16, length, [0] * batch, extra=80)
+    check_attention(dev, stream, pool, table, start, length, q, D.BF16, 4)
 
 
 def test_long_step_is_the_same_twice(dev, stream):

@@ -40,13 +40,15 @@ int sample_go(const void* logits, int32_t* tokens, uint32_t rows, uint32_t vocab
       return fail(TH_KERNEL_ERROR, "sample: grid too large");
     void* sums = nullptr;
     th::ScratchHold hold;
-    TH_TRY(th::stream_scratch(s, sizeof(th::smp::PartSum) * rows * parts, &sums, &hold));
-    auto* ps = static_cast<th::smp::PartSum*>(sums);
-    hipLaunchKernelGGL((th::smp::sample_parts<DT>), dim3(rows * parts), dim3(256), 0, s, logits, ps,
-                       vocab, stride, temperature, parts);
-    hipLaunchKernelGGL((th::smp::sample_pick<DT>), dim3(rows), dim3(th::smp::NT), 0, s, logits,
-                       tokens, vocab, stride, uniform, temperature, ps, parts);
-    return launch_status("sample launch");
+    // (without memory for them the rows stay whole)
+    if (th::try_stream_scratch(s, sizeof(th::smp::PartSum) * rows * parts, &sums, &hold)) {
+      auto* ps = static_cast<th::smp::PartSum*>(sums);
+      hipLaunchKernelGGL((th::smp::sample_parts<DT>), dim3(rows * parts), dim3(256), 0, s, logits,
+                         ps, vocab, stride, temperature, parts);
+      hipLaunchKernelGGL((th::smp::sample_pick<DT>), dim3(rows), dim3(th::smp::NT), 0, s, logits,
+                         tokens, vocab, stride, uniform, temperature, ps, parts);
+      return launch_status("sample launch");
+    }
   }
   using std::integral_constant;
   if (blocks <= 1024 * 2) go(integral_constant<int, 2>{});
