@@ -318,7 +318,7 @@ int th_kv_cache_read(const th_kv_pages* pages, const th_kv_batch* seqs, void* k,
  * num_heads * head_dim and a multiple of 8), O the same, dense, and not in Q's memory.  dtype is
  * F16 or BF16; the cache is of that dtype, or E4M3 or I8.  num_heads is a multiple of
  * num_kv_heads.  Scores, softmax and sums are f32; weights are rounded to dtype, with an 8-bit
- * cache weight times scale to f16.  A token that sees nothing gives zeros.  What a token does not
+ * cache weight times scale to f16 (or to two values of it that add up to more).  A token that sees nothing gives zeros.  What a token does not
  * see has no effect on it, NaN and infinities included.
  * The work is split by the lengths on the device, so one captured call serves any lengths; the
  * parts' sums go to `workspace`, device memory of at least th_attention_paged_workspace_size

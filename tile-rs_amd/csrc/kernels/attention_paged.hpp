@@ -35,6 +35,21 @@ __device__ __forceinline__ uint32_t pack2h(float lo, float hi) {
   }
 }
 
+// What pack2h's rounding left of a pair, rounded itself.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2h_rest(float lo, float hi, uint32_t xy) {
+  if constexpr (DT == kBF16) {
+    lo -= __uint_as_float(xy << 16);
+    hi -= __uint_as_float(xy & 0xffff0000u);
+  } else {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 x = __builtin_bit_cast(h2, xy);
+    lo -= static_cast<float>(x[0]);
+    hi -= static_cast<float>(x[1]);
+  }
+  return pack2h<DT>(lo, hi);
+}
+
 // a + x + y of a pair as pack2h rounded it.  (Weights are summed as the product with V takes them,
 // so that the mean is one of weights that sum to 1: a token that has all the weight gives its
 // values exactly.)
@@ -131,7 +146,8 @@ __device__ __forceinline__ int32_t paged_checked(const PagedSeqs& s, int32_t id)
 // the largest and less, and a tile that sees such a scale is summed again by SlowRow.)
 constexpr float kLeastExp = -100.0f, kMostExp = 90.0f;
 __device__ __forceinline__ float scale_exp(float most) {
-  return most > 0.0f ? static_cast<float>(__builtin_amdgcn_frexp_expf(most)) : kLeastExp;
+  const float e = most < INFINITY ? static_cast<float>(__builtin_amdgcn_frexp_expf(most)) : 128.0f;
+  return most > 0.0f ? e : kLeastExp;
 }
 
 // Whether a NaN or an infinity is among the 16 bytes.
@@ -375,6 +391,10 @@ struct RowsTile {
   // Weights times codes' scales, and the codes of V, which f16 holds exactly, go into the product
   // as f16 whatever Q is: 8 times less rounding than bf16, at 0 to 4% of the time.
   static constexpr int PT = kCodes ? static_cast<int>(kF16) : DT;
+  // Tiles of 16 rows, whose time goes to the cache's bytes, take a weight in two parts of 16 bits,
+  // with a product each, unless it has more bits than O as it is: O's own rounding is then all
+  // that shows.
+  static constexpr bool kTwo = MT == 1 && PT == DT;
   static constexpr int ESZ = cache_size<CT>();
   static constexpr int TR = 16 * MT;
   static constexpr int NS = HD / 32;             // K fragments (32 values deep) of a position
@@ -489,7 +509,8 @@ struct RowsTile {
   }
 
   // acc += V^T . P^T, V from LDS.
-  static __device__ __forceinline__ void pv(const char* lds, const u32x4 (&pf)[MT], Sums& y) {
+  static __device__ __forceinline__ void pv(const char* lds, const u32x4 (&pf)[MT],
+                                            const u32x4& rest, Sums& y) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
     const uint32_t r = 4 * g + (l16 >> 2);
 #pragma unroll
@@ -501,6 +522,8 @@ struct RowsTile {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
         y.acc[i][c] = mfma16x16x32<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[i], y.acc[i][c]);
+      if constexpr (kTwo)
+        y.acc[0][c] = mfma16x16x32<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, rest, y.acc[0][c]);
     }
   }
 
@@ -597,7 +620,7 @@ struct RowsTile {
         pages(a, b, base + 2 * rows::UNIT, c.held, next);
       }
 
-      u32x4 pf[MT];
+      u32x4 pf[MT], rest;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         // of positions base + 16 (x / 4) + 4 g + x % 4, the row sees those below lim[x / 4]
@@ -647,10 +670,8 @@ struct RowsTile {
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           p[x] = exp2_fast(s[i][x >> 2][x & 3] - mu);
-          if constexpr (kCodes) {
-            y.l[i] += p[x];
-            p[x] *= w[x];
-          }
+          if constexpr (kCodes || kTwo) y.l[i] += p[x];
+          if constexpr (kCodes) p[x] *= w[x];
         }
         if (moved) {
 #pragma unroll
@@ -660,12 +681,16 @@ struct RowsTile {
         }
         pf[i] = u32x4{pack2h<PT>(p[0], p[1]), pack2h<PT>(p[2], p[3]), pack2h<PT>(p[4], p[5]),
                       pack2h<PT>(p[6], p[7])};
-        if constexpr (!kCodes) {
+        if constexpr (kTwo) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            rest[x] = pack2h_rest<PT>(p[2 * x], p[2 * x + 1], pf[i][x]);
+        } else if constexpr (!kCodes) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) y.l[i] = add_pair<DT>(pf[i][x], y.l[i]);
         }
       }
-      pv(vlds, pf, y);
+      pv(vlds, pf, rest, y);
     }
 
     // the four waves' sums
